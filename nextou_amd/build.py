@@ -22,6 +22,7 @@ HIP_FLAGS = [
     "-ffp-contract=off",                         # explicit fmaf only: bit-exact vs the oracle
     "-fhip-fp32-correctly-rounded-divide-sqrt",  # IEEE divide / sqrt in knn_prep
     "-munsafe-fp-atomics",                       # hardware f32 atomic add (coarse-grained HBM)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",   # no v_pk_*_f32: some of their forms have given wrong results (the host pass ignores this, with a warning)
     "-Wall", "-Wno-unused-function",
 ]
 
