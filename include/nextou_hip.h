@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define NEXTOU_ABI_VERSION 14
+#define NEXTOU_ABI_VERSION 15
 
 #define NEXTOU_EINVAL   (-1)  /* bad argument (null pointer, non-positive size, k > M ...) */
 #define NEXTOU_ENOSPACE (-2)  /* workspace too small */
@@ -589,6 +589,50 @@ int nextou_stem_bwd(const float* x, const float* gy, const uint32_t* act_mask, c
                     const float* save_mean, const float* save_invstd, const double* moments, float* gweight, float* ggamma,
                     float* gbeta, void* workspace, size_t workspace_bytes, int B, int D, int H, int W, int C, int Cpad,
                     float slope, nextou_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * K10  point-wise products with their epilogue (ABI v15): the 1x1 convolution / linear layer of a block with its bias, its activation
+ * and its shortcut in one launch, and the gradients, in float32 (dtype 0), bfloat16 (1) and float16 (2).  Replaces conv -> act (-> add)
+ * of the reference's BasicConv without a norm (torch_nn.py:66-92) and, with the norm's running statistics folded into w and bias,
+ * conv -> norm -> act (-> add) of FFN / fc1 / fc2 in evaluation (NexToU_Encoder_Decoder.py:368-390, :710-720, :833-842).
+ *   z[p, g*N + n] = sum_k x[p, g*K + k] * w[g*N + n, k] + bias[g*N + n]        y = act(z) + residual
+ *   act: 0 none, 1 relu, 2 leaky relu (slope), 3 gelu (z Phi(z)), 4 hardswish.  Any P, N, K >= 1, any element-aligned pointers and row
+ *   strides (ldx and ldr may be 0: one row for all; ldy >= groups * N); columns are dense, w is dense (groups * N, K).  bias and residual may be NULL; bias
+ *   is float32 when bias_f32, else of the rows' type.  Sums in float32, each output rounded once.
+ *   pre (may be NULL): z for the backward, dense (P, groups * N) — float32 for float32 rows, float16 for both 16-bit types, clamped to
+ *   its range, a positive z never rounded to zero.
+ * nextou_linear_act_bwd   dz = gy * act'(z) (rounded to the rows' type for the products, unrounded in gb), gx = dz w, gw = dz^T x,
+ *   gb = sum_p dz; any of gx (dense), gw (dense, like w), gb (float32 when gb_f32, else the rows' type) may be NULL.  saved_kind: 0 none
+ *   (act 0), 1 `saved` is the forward's pre, 2 `saved` is the forward's y, dense (relu, leaky relu with slope >= 0 and no residual: its sign is z's).
+ *   Sums over points in a fixed order: bit-reproducible.
+ * workspace: the matching _workspace call's bytes, contents irrelevant; one per call in flight.
+ * ---------------------------------------------------------------------------------------- */
+int nextou_linear_act_fwd_workspace(int64_t P, int N, int K, int groups, int dtype, size_t* bytes);
+int nextou_linear_act_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre, void* workspace,
+                          size_t workspace_bytes, int64_t P, int N, int K, int groups, int64_t ldx, int64_t ldr, int64_t ldy, int dtype,
+                          int bias_f32, int act, float slope, nextou_stream_t stream);
+int nextou_linear_act_bwd_workspace(int64_t P, int N, int K, int groups, int dtype, int act, int want_gx, int want_gw, int want_gb,
+                                    size_t* bytes);
+int nextou_linear_act_bwd(const void* gy, const void* x, const void* w, const void* saved, int saved_kind, void* gx, void* gw, void* gb,
+                          void* workspace, size_t workspace_bytes, int64_t P, int N, int K, int groups, int64_t ldg, int64_t ldx, int dtype,
+                          int gb_f32, int act, float slope, nextou_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
+ * K11  the global norm of a list of gradients, and the clip (ABI v15): clip_grad_norm_(parameters, max_norm, norm) of nnU-Net's
+ * train_step for any mixture of types and any optimizer (K-glue's nextou_grad_norm_clip_coef is the float32 form on its way into SGD).
+ *   table_host   HOST int64 [n_tensors][3]: device pointer (a multiple of the element size), element count > 0, type (0 float32,
+ *                1 bfloat16, 2 float16); read during the call, its values travel as launch arguments.  Each tensor is a dense run of
+ *                elements; for the clip no two may overlap.
+ *   norm         0: max |g| (NaN if any is), 1: sum |g|, 2: sqrt(sum g^2) — float64 sums in a fixed order
+ *   norm_coef    out, 2 floats: the norm, and min(1, max_norm / (norm + 1e-6)) (NaN for a NaN norm)
+ * nextou_multi_norm leaves the gradients alone; nextou_multi_clip multiplies them by norm_coef[1] in place (rounded once each).
+ * workspace: nextou_multi_norm_workspace bytes, contents irrelevant; one per call in flight.
+ * ---------------------------------------------------------------------------------------- */
+int nextou_multi_norm_workspace(int n_tensors, size_t* bytes);
+int nextou_multi_norm(const int64_t* table_host, int n_tensors, int norm, float max_norm, void* workspace, size_t workspace_bytes,
+                      float* norm_coef, nextou_stream_t stream);
+int nextou_multi_clip(const int64_t* table_host, int n_tensors, int norm, float max_norm, void* workspace, size_t workspace_bytes,
+                      float* norm_coef, nextou_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -12,6 +12,8 @@ Each operator is the fused replacement of a run of ATen ops in the reference (SU
                        (reference loss/bti_loss.py:132-134, 76-117)
 ``norm_act``           batch_norm | instance_norm -> leaky_relu (reference torch_nn.py:84-90,
                        NexToU_Encoder_Decoder.py:384-390 and the conv stages' norm -> nonlin)
+``linear_act``         conv 1x1 / linear -> bias -> activation (-> + shortcut), any width, float32 and 16 bits
+                       (reference torch_nn.py:66-92 without a norm; NexToU_Encoder_Decoder.py:384-390 in evaluation)
 =====================  =====================================================================
 
 Device tensors go to the HIP kernels through the C-ABI (plain pointers + the current HIP stream).
@@ -33,7 +35,7 @@ from . import _lib
 __all__ = [
     "knn_graph", "pairwise_sq_distance", "edge_index_from_nn_idx", "mr_aggregate", "gather_neighbors",
     "argmax_labels", "bti_critical_map", "critical_cross_entropy", "norm_act", "install_cpu_checker", "IndexTape",
-    "index_tape", "window_gather", "window_scatter", "pool_rows", "cell_scatter",
+    "index_tape", "window_gather", "window_scatter", "pool_rows", "cell_scatter", "linear_act", "pointwise_act",
 ]
 
 
@@ -889,6 +891,48 @@ class _HipBackend:
         return gx
 
 
+    # ---- K10: point-wise products with bias, activation and shortcut in the epilogue ----
+    @staticmethod
+    def linear_act_fwd(x, w, bias, residual, act, slope, groups, want_pre):
+        """x (P, groups*K) rows with dense columns, w (groups*N, K) dense -> (y (P, groups*N) dense, z for the backward | None)."""
+        import ctypes
+        L_ = _lib.lib()
+        P, (C, K) = x.shape[0], w.shape
+        N, code = C // groups, _LINEAR_TYPES[x.dtype]
+        need = ctypes.c_size_t(0)
+        with torch.cuda.device(x.device):
+            _lib.check(L_.nextou_linear_act_fwd_workspace(P, N, K, groups, code, ctypes.byref(need)), "linear_act_fwd_workspace")
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
+            y = torch.empty((P, C), dtype=x.dtype, device=x.device)
+            pre = torch.empty((P, C), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device) if want_pre else None
+            rc = L_.nextou_linear_act_fwd(x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(pre), _ptr(ws), need.value,
+                                          P, N, K, groups, x.stride(0), 0 if residual is None else residual.stride(0), C, code,
+                                          int(bias is not None and bias.dtype == torch.float32), act, slope, _stream_ptr(x.device))
+        _lib.check(rc, "linear_act_fwd")
+        return y, pre
+
+    @staticmethod
+    def linear_act_bwd(gy, x, w, saved, saved_kind, act, slope, groups, want_gx, want_gw, gb_dtype):
+        """(gx (P, groups*K), gw like w, gb (groups*N,)), each None when not wanted; gb_dtype None: no bias gradient."""
+        import ctypes
+        L_ = _lib.lib()
+        P, (C, K) = x.shape[0], w.shape
+        N, code = C // groups, _LINEAR_TYPES[x.dtype]
+        need = ctypes.c_size_t(0)
+        with torch.cuda.device(x.device):
+            _lib.check(L_.nextou_linear_act_bwd_workspace(P, N, K, groups, code, act, int(want_gx), int(want_gw), int(gb_dtype is not None),
+                                                          ctypes.byref(need)), "linear_act_bwd_workspace")
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
+            gx = torch.empty((P, groups * K), dtype=x.dtype, device=x.device) if want_gx else None
+            gw = torch.empty((C, K), dtype=x.dtype, device=x.device) if want_gw else None
+            gb = torch.empty((C,), dtype=gb_dtype, device=x.device) if gb_dtype is not None else None
+            rc = L_.nextou_linear_act_bwd(gy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(saved), saved_kind, _ptr(gx), _ptr(gw), _ptr(gb),
+                                          _ptr(ws), need.value, P, N, K, groups, gy.stride(0), x.stride(0), code,
+                                          int(gb_dtype == torch.float32), act, slope, _stream_ptr(x.device))
+        _lib.check(rc, "linear_act_bwd")
+        return gx, gw, gb
+
+
 def _logit_strides(logits, nl, V):
     """(stride_l, stride_v) of dense logits (B, L, *sp): (1, L) when stored channels-last (even class count: the rows kernels read
     8-byte pairs), else (V, 1) — the caller made NCDHW-dense tensors of everything else (:func:`_logits_in_place`)."""
@@ -1732,6 +1776,106 @@ def stem_block(x: torch.Tensor, conv: torch.nn.Module, norm: torch.nn.Module) ->
     return _StemBlock.apply(x, conv.weight, pre_bias, norm.weight, norm.bias, norm.running_mean if keep_running else None,
                             norm.running_var if keep_running else None, bool(use_batch_stats), float(factor), float(norm.eps),
                             float(norm.negative_slope), int(c_pad))
+
+
+_LINEAR_TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_LINEAR_ACTS = {"none": 0, "relu": 1, "leakyrelu": 2, "gelu": 3, "hswish": 4, "hardswish": 4}
+
+
+def _as_rows(t: torch.Tensor) -> torch.Tensor:
+    """(..., C) -> (P, C) with dense columns and one row stride: a view where the strides allow one (an expanded row included), else a copy."""
+    rows = t.reshape(-1, t.shape[-1])
+    return rows if rows.shape[1] == 1 or rows.stride(1) == 1 else rows.contiguous()
+
+
+class _LinearAct(torch.autograd.Function):
+    """K10 over rows.  What the backward needs of z: nothing without an activation; the output itself where its sign is z's (ReLU and
+    LeakyReLU without a shortcut; float16 apart, whose small positive values can round to zero); else z, written by the same launch."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, slope, groups, training):
+        be = _backend_for(x)
+        if x.numel() == 0:
+            ctx.save_for_backward(x, weight, None)
+            ctx.conf = (None, act, slope, groups, None if bias is None else bias.dtype)
+            return x.new_empty(x.shape[:-1] + (weight.shape[0],))
+        x2, w2 = _as_rows(x), weight.contiguous()
+        sign = act == 1 or (act == 2 and slope >= 0.0)
+        kind = 0 if act == 0 or not training else (2 if sign and residual is None and x.dtype != torch.float16 else 1)
+        y, pre = be.linear_act_fwd(x2, w2, bias, None if residual is None else _as_rows(residual), act, slope, groups, kind == 1)
+        y = y.view(x.shape[:-1] + (w2.shape[0],))
+        if training:
+            ctx.save_for_backward(x, weight, pre if kind == 1 else (y if kind == 2 else None))
+            ctx.conf = (kind, act, slope, groups, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, saved = ctx.saved_tensors
+        kind, act, slope, groups, bias_dtype = ctx.conf
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        gx = gw = gb = None
+        if kind is None:          # no rows
+            gx, gw = torch.zeros_like(x), torch.zeros_like(weight, memory_format=torch.contiguous_format)
+            gb = None if bias_dtype is None else torch.zeros(weight.shape[0], dtype=bias_dtype, device=x.device)
+        elif want_x or want_w or want_b:
+            gx, gw, gb = _backend_for(x).linear_act_bwd(
+                _as_rows(gy), _as_rows(x), weight.contiguous(), None if saved is None else saved.reshape(-1, weight.shape[0]), kind, act,
+                slope, groups, want_x, want_w, bias_dtype if want_b else None)
+        return (None if gx is None else gx.view(x.shape), None if gw is None else gw.view(weight.shape), gb,
+                gy if ctx.needs_input_grad[3] else None, None, None, None, None)
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+               act: str = "none", negative_slope: float = 0.01, groups: int = 1) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` in one launch, with its gradients (K10, csrc/linear_act.hip).
+
+    x (..., groups * K); weight (groups * N, K); bias (groups * N,) or None; residual (..., groups * N) or None -> (..., groups * N).
+    ``groups`` > 1: channel group g of the output sees channel group g of the input, as in a grouped 1x1 convolution.  ``act``: "none",
+    "relu", "leakyrelu" (``negative_slope``), "gelu" (the exact one) or "hswish".
+
+    float32, bfloat16 or float16; all tensors of one type, except that the bias may be float32 beside 16-bit rows.  Sums are held in
+    float32 and every output and gradient is rounded once (with an activation in 16 bits, so is d loss / d z on its way into the two
+    gradient products).  Under autocast the tensors are cast to the autocast type first.  Any sizes and any strides: columns that are not
+    dense are copied, an expanded row is read as it is.  Gradients are bit-reproducible; there is no double backward.
+    ValueError / TypeError for shapes, types or devices that do not fit."""
+    if act not in _LINEAR_ACTS:
+        raise ValueError("linear_act: act %r is none of %s" % (act, ", ".join(sorted(_LINEAR_ACTS))))
+    groups = int(groups)
+    if weight.dim() != 2 or x.dim() < 1 or groups < 1 or weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[0] % groups or \
+            x.shape[-1] != groups * weight.shape[1]:
+        raise ValueError("linear_act: x %s and weight %s do not fit %d group(s)" % (tuple(x.shape), tuple(weight.shape), groups))
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError("linear_act: bias %s for %d output channels" % (tuple(bias.shape), weight.shape[0]))
+    if residual is not None and tuple(residual.shape) != tuple(x.shape[:-1]) + (weight.shape[0],):
+        raise ValueError("linear_act: residual %s for an output of %s" % (tuple(residual.shape), tuple(x.shape[:-1]) + (weight.shape[0],)))
+    given = [t for t in (x, weight, bias, residual) if t is not None]
+    if any(t.device != x.device for t in given):
+        raise ValueError("linear_act: tensors on %s" % ", ".join(sorted({str(t.device) for t in given})))
+    if x.is_cuda and torch.is_autocast_enabled("cuda") and all(t.dtype in _LINEAR_TYPES for t in given):
+        dt = torch.get_autocast_dtype("cuda")
+        x, weight = x.to(dt), weight.to(dt)
+        bias = bias if bias is None or bias.dtype == torch.float32 else bias.to(dt)
+        residual = None if residual is None else residual.to(dt)
+    if x.dtype not in _LINEAR_TYPES or weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype) or \
+            (bias is not None and bias.dtype not in (x.dtype, torch.float32)):
+        raise TypeError("linear_act: float32, bfloat16 or float16 tensors of one type (a float32 bias apart), got %s" %
+                        ", ".join(str(t.dtype) for t in given))
+    training = torch.is_grad_enabled() and any(t.requires_grad for t in given)
+    return _LinearAct.apply(x, weight, None if bias is None else bias.contiguous(), residual, _LINEAR_ACTS[act], float(negative_slope), groups,
+                            training)
+
+
+def pointwise_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                  act: str = "none", negative_slope: float = 0.01, groups: int = 1) -> torch.Tensor:
+    """:func:`linear_act` on a volume: x (B, groups * K, *spatial), weight (groups * N, K, 1[, 1[, 1]]) as a convolution stores it, residual
+    (B, groups * N, *spatial) -> (B, groups * N, *spatial) in channels-last memory.  Channels-last inputs are read in place, others copied."""
+    if x.dim() < 3 or weight.dim() != x.dim() or any(k != 1 for k in weight.shape[2:]):
+        raise ValueError("pointwise_act: x %s with weight %s is no kernel-1 convolution" % (tuple(x.shape), tuple(weight.shape)))
+    last = (0,) + tuple(range(2, x.dim())) + (1,)
+    y = linear_act(x.permute(last), weight.flatten(1), bias, None if residual is None else residual.permute(last), act, negative_slope, groups)
+    return y.permute((0, x.dim() - 1) + tuple(range(1, x.dim() - 1)))
 
 
 PW_GEMM_DEFAULT = "0"

@@ -161,7 +161,8 @@ class StandaloneTrainerBase:
         if hasattr(self.optimizer, "clip_and_step"):
             self.optimizer.clip_and_step(12)
         else:
-            torch.nn.utils.clip_grad_norm_(self.network.parameters(), 12)
+            from .optim import clip_grad_norm_
+            clip_grad_norm_(self.network.parameters(), 12)
             self.optimizer.step()
         return loss.detach()
 

@@ -13,17 +13,23 @@ multiply-add here, a separately rounded product there — the same spread as bet
 variants).  Anything the kernels do not take (CPU or non-float32 parameters, sparse gradients, dampening, maximize) goes through
 torch's implementation, unchanged — ``last_path`` / ``last_reason`` say which ran and why; a gradient stored in another element order
 than its parameter is copied into the parameter's order first.
+
+``clip_grad_norm_`` and ``grad_norm`` are the clip alone, for any optimizer: gradients of float32, bfloat16 and float16 in one list, the 2-, 1-
+or maximum norm, two launches whatever the tensor count (csrc/grad_norm.hip, ABI v15).
 """
 from __future__ import annotations
 
+import array
+import ctypes
+import math
 import os
-from typing import List, Optional
+from typing import Iterable, List, Optional, Union
 
 import torch
 
 from . import _lib
 
-__all__ = ["ClipSGD"]
+__all__ = ["ClipSGD", "clip_grad_norm_", "grad_norm"]
 
 _CHUNK = 16384          # elements per workgroup (64 KB of each tensor)
 
@@ -72,13 +78,118 @@ class _on_device:
         return False
 
 
+_NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORM_CODES = {math.inf: 0, 1.0: 1, 2.0: 2}
+_LAST = {4: torch.channels_last, 5: torch.channels_last_3d}
+
+
+def _norm_code(norm_type) -> int:
+    code = _NORM_CODES.get(float(norm_type))
+    if code is None:
+        raise ValueError("the norm of gradients is the 1-, 2- or maximum (inf) norm, not %r" % (norm_type,))
+    return code
+
+
+def _flat_run(t: torch.Tensor) -> bool:
+    return t.is_contiguous() or (t.dim() in _LAST and t.is_contiguous(memory_format=_LAST[t.dim()])) or _dense(t)
+
+
+def _norm_rows(tensors: List[torch.Tensor], in_place: bool):
+    """(host table, [(tensor, its dense copy)]) of the tensors that have elements; everything the kernels do not take is refused here."""
+    device, vals, copies = tensors[0].device, array.array("q"), []
+    for t in tensors:
+        code = _NORM_TYPES.get(t.dtype)
+        if code is None or t.layout is not torch.strided:
+            raise TypeError("gradient norm: dense float32, bfloat16 or float16 gradients, got %s %s" % (t.layout, t.dtype))
+        if t.device != device:
+            raise ValueError("gradient norm: gradients on %s and %s" % (device, t.device))
+        n = t.numel()
+        if n == 0:
+            continue
+        if not _flat_run(t):
+            if in_place and any(a < b for a, b in _strides_and_reach(t)):
+                raise ValueError("gradient norm: a gradient of shape %s and strides %s overlaps itself" % (tuple(t.shape), t.stride()))
+            copies.append((t, t.contiguous()))
+            t = copies[-1][1]
+        vals.extend((t.data_ptr(), n, code))
+    return vals, copies
+
+
+def _strides_and_reach(t: torch.Tensor):
+    """Per dimension longer than one, by ascending stride: (stride, elements that the smaller dimensions span); a stride below the span overlaps."""
+    reach = 1
+    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        yield stride, reach
+        reach += stride * (n - 1)
+
+
+def _multi_norm(tensors: List[torch.Tensor], code: int, max_norm: float, scale: bool) -> torch.Tensor:
+    """float32 (norm, clip factor) of device tensors; ``scale`` multiplies them by the factor in place."""
+    device = tensors[0].device
+    with _on_device(device):
+        vals, copies = _norm_rows(tensors, scale)
+        if not vals:
+            return torch.zeros(2, device=device)          # only empty tensors
+        n, L = len(vals) // 3, _lib.lib()
+        need = ctypes.c_size_t(0)
+        _lib.check(L.nextou_multi_norm_workspace(n, ctypes.byref(need)), "multi_norm_workspace")
+        ws = torch.empty((need.value,), dtype=torch.uint8, device=device)
+        out = torch.empty((2,), dtype=torch.float32, device=device)
+        call = L.nextou_multi_clip if scale else L.nextou_multi_norm
+        _lib.check(call(vals.buffer_info()[0], n, code, max_norm, ws.data_ptr(), need.value, out.data_ptr(), _stream_of(device)),
+                   "multi_clip" if scale else "multi_norm")
+        if scale:
+            for t, dense in copies:
+                t.copy_(dense)
+    return out
+
+
+@torch.no_grad()
+def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
+    """The ``norm_type``-norm (1, 2 or inf) of all elements of ``tensors`` taken together, as a 0-dim float32 tensor on their device (no host
+    synchronisation): what ``torch.nn.utils.get_total_norm`` returns, for float32 / bfloat16 / float16 tensors in one list, with float64 sums
+    in a fixed order.  NaN if any element is.  An empty list gives 0.  TypeError / ValueError for other types and mixed devices."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    code = _norm_code(norm_type)
+    if not tensors:
+        return torch.tensor(0.0)
+    if not tensors[0].is_cuda:
+        return torch.nn.utils.get_total_norm(tensors, float(norm_type)).float()
+    return _multi_norm(tensors, code, math.inf, False)[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False, foreach: Optional[bool] = None) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` for gradients on the GPU in two launches: every gradient times ``min(1, max_norm / (norm + 1e-6))``, in place,
+    rounded once; returns the norm before the clip (0-dim float32, no host synchronisation unless ``error_if_nonfinite``).
+
+    Gradients may be float32, bfloat16 and float16 in one list, of any dense layout (others are copied and written back).  A norm that is
+    infinite or NaN scales as in torch: to zeros and NaN.  No two gradients may share memory (a parameter listed twice: RuntimeError).
+    CPU gradients go through torch's implementation; ``foreach`` is accepted for its signature.  Capturable: the gradients' addresses and
+    ``max_norm`` are those of the capture."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    code, max_norm = _norm_code(norm_type), float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("clip_grad_norm_: max_norm %g" % max_norm)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    if not grads[0].is_cuda:
+        return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite, foreach)
+    if error_if_nonfinite:
+        norm = _multi_norm(grads, code, max_norm, False)[0]
+        if not math.isfinite(norm.item()):
+            raise RuntimeError("The total norm of order %s for gradients from `parameters` is non-finite, so it cannot be clipped." % norm_type)
+    return _multi_norm(grads, code, max_norm, True)[0]
+
+
 class _Table:
     """Device table + chunk list + workspace of one set of (parameter, gradient, buffer) tensors.  Immutable once built: the values
     travel as kernel arguments (nextou_device_write_i64), so a captured hipGraph keeps rewriting — and its kernels keep reading — the
     table it was captured with; nothing on the host is read at replay and no pinned allocation happens inside a capture."""
 
     def __init__(self, rows: List[tuple], device: torch.device):
-        import ctypes
         flat, chunks, total = [], [], 0
         for i, (p, g, m, n) in enumerate(rows):
             flat.extend((p, g, m, n))
@@ -192,6 +303,18 @@ class ClipSGD(torch.optim.SGD):
             self._retired.append(t)               # the captured graph's kernels keep reading this table after a later step replaced it
         return t
 
+    @staticmethod
+    def _norm_of_groups(rows, device, max_norm):
+        vals = array.array("q", [v for _, g, _, n in rows for v in (g, n, 0)])
+        L, need = _lib.lib(), ctypes.c_size_t(0)
+        with _on_device(device):
+            _lib.check(L.nextou_multi_norm_workspace(len(rows), ctypes.byref(need)), "multi_norm_workspace")
+            ws = torch.empty((need.value,), dtype=torch.uint8, device=device)
+            out = torch.empty((2,), dtype=torch.float32, device=device)
+            _lib.check(L.nextou_multi_norm(vals.buffer_info()[0], len(rows), 2, float(max_norm), ws.data_ptr(), need.value, out.data_ptr(),
+                                           _stream_of(device)), "multi_norm")
+        return out
+
     # ---------------------------------------------------------------------------------------------------------------
     @torch.no_grad()
     def _own_step(self, max_norm: Optional[float]):
@@ -204,14 +327,17 @@ class ClipSGD(torch.optim.SGD):
             return None if max_norm is None else torch.zeros(())
         plans = {gi: self._plan(self.param_groups[gi]) for gi in groups_with_grads}
         why = [pl for pl in plans.values() if isinstance(pl, str)]
-        if not why and max_norm is not None and len(plans) != 1:
-            why = ["the clip's norm spans %d parameter groups (the kernels take one table)" % len(plans)]
+        if not why and max_norm is not None and len({device for _, device in plans.values()}) != 1:
+            why = ["the clip's norm spans several devices"]
         self.last_reason = why[0] if why else None
         if why:
             return NotImplemented
         live = sorted(plans.items())
         L = _lib.lib()
-        norm = None
+        norm = shared = None
+        if max_norm is not None and len(live) > 1:      # one norm over all groups (K11); each group's update reads its factor
+            shared = self._norm_of_groups([r for _, (rows, _) in live for r in rows], live[0][1][1], max_norm)
+            norm = shared[0]
         for gi, (rows, device) in live:
             group = self.param_groups[gi]
             t = self._table(gi, rows, device)
@@ -219,13 +345,14 @@ class ClipSGD(torch.optim.SGD):
             lr_dev = lr.data_ptr() if isinstance(lr, torch.Tensor) else None
             with _on_device(device):
                 stream = _stream_of(device)
-                if max_norm is not None:
+                if max_norm is not None and shared is None:
                     _lib.check(L.nextou_grad_norm_clip_coef(t.table.data_ptr(), t.n_tensors, t.chunks.data_ptr(), t.n_chunks, _CHUNK,
                                                             t.total, t.partial.data_ptr(), float(max_norm), t.norm_coef.data_ptr(),
                                                             stream), "grad_norm_clip_coef")
                     norm = t.norm_coef[0]
+                coef = None if max_norm is None else (t.norm_coef if shared is None else shared)
                 _lib.check(L.nextou_clip_sgd_update(t.table.data_ptr(), t.n_tensors, t.chunks.data_ptr(), t.n_chunks, _CHUNK, t.total,
-                                                    t.norm_coef.data_ptr() if max_norm is not None else None,
+                                                    coef.data_ptr() if coef is not None else None,
                                                     0.0 if lr_dev else float(lr), lr_dev, float(group["momentum"]),
                                                     float(group["weight_decay"]), int(bool(group["nesterov"])), stream),
                            "clip_sgd_update")

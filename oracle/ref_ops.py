@@ -9,6 +9,8 @@ travel to the GPU box).  Each function cites the reference lines it follows.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -152,6 +154,52 @@ def norm_act_bwd_ref(x, gy, weight, bias, save_mean, save_invstd, training, slop
     return gx, gw, gb
 
 
+def _act64(z, act, slope):
+    """value and slope of nextou_linear_act's activations (0 none, 1 relu, 2 leaky relu, 3 gelu, 4 hardswish) in float64"""
+    if act == 1:
+        return torch.where(z <= 0, torch.zeros_like(z), z), (z > 0).double()
+    if act == 2:
+        return torch.where(z > 0, z, z * slope), torch.where(z > 0, 1.0, float(slope)).double()
+    if act == 3:
+        phi = 0.5 * torch.special.erfc(-z / math.sqrt(2.0))
+        return z * phi, phi + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi)
+    if act == 4:
+        return z * (z + 3).clamp(0, 6) / 6, torch.where(z <= -3, 0.0, torch.where(z >= 3, 1.0, (2 * z + 3) / 6))
+    return z, torch.ones_like(z)
+
+
+def _grouped64(a, b, groups):
+    """(P, groups*A), (groups*B, A) -> (P, groups*B): a_g b_g^T per group"""
+    ag, bg = a.double().reshape(a.shape[0], groups, -1), b.double().reshape(groups, b.shape[0] // groups, -1)
+    return torch.stack([ag[:, g] @ bg[g].t() for g in range(groups)], 1).reshape(a.shape[0], -1)
+
+
+def linear_act_fwd_ref(x, w, bias, residual, act, slope, groups, want_pre):
+    """float64 restatement of nextou_linear_act_fwd -> (y in x's type, z in float64 | None)"""
+    z = _grouped64(x, w, groups)
+    if bias is not None:
+        z = z + bias.double()
+    y = _act64(z, act, slope)[0]
+    if residual is not None:
+        y = y + residual.double()
+    return y.to(x.dtype), z if want_pre else None
+
+
+def linear_act_bwd_ref(gy, x, w, saved, saved_kind, act, slope, groups, want_gx, want_gw, gb_dtype):
+    """float64 restatement of nextou_linear_act_bwd"""
+    dz = gy.double()
+    if saved_kind:
+        dz = dz * _act64(saved.double(), act, slope)[1]
+    n, k = w.shape[0] // groups, w.shape[1]
+    wt = w.reshape(groups, n, k).transpose(1, 2).reshape(groups * k, n)
+    gx = _grouped64(dz, wt, groups).to(x.dtype) if want_gx else None
+    gw = None
+    if want_gw:
+        dg, xg = dz.reshape(-1, groups, n), x.double().reshape(-1, groups, k)
+        gw = torch.cat([dg[:, g].t() @ xg[:, g] for g in range(groups)]).to(w.dtype)
+    return gx, gw, None if gb_dtype is None else dz.sum(0).to(gb_dtype)
+
+
 class TorchRefBackend:
     """Backend protocol of nextou_amd.graph_ops with the reference's op sequence (CPU baseline)."""
 
@@ -254,6 +302,9 @@ class TorchRefBackend:
     @staticmethod
     def channel_sum(x, channels_last=False):
         return x.double().sum(dim=[0] + list(range(2, x.dim()))).float()
+
+    linear_act_fwd = staticmethod(linear_act_fwd_ref)
+    linear_act_bwd = staticmethod(linear_act_bwd_ref)
 
 
 # ----------------------------------------------------------------------------------------------
