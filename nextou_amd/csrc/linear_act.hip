@@ -5,41 +5,110 @@
 //
 // Sums are held in float32; y, dz (16-bit types only: the matrix units read 16-bit operands) and the gradients are rounded once each.
 #include "common.h"
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 
 namespace nextou {
 namespace {
 
 using bf16_t = __bf16;
 using f16_t = _Float16;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
 
 enum Act { kActNone = 0, kActRelu = 1, kActLeaky = 2, kActGelu = 3, kActHardswish = 4 };
 
+// ---- activations --------------------------------------------------------------------------------------------------------------------
 constexpr float kInvSqrt2 = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
 
+// Phi(z), and e = exp(-z^2 / 2) beside it.  float32 rows: the library's erfc (relative accuracy in both tails).  16-bit rows: Abramowitz and
+// Stegun 7.1.26 (|error| <= 1.5e-7 of erf), five multiply-adds, one exp and one reciprocal instead of some forty instructions.
+template <bool FAST>
+__device__ __forceinline__ float normal_cdf(float z, float* e) {
+    if constexpr (FAST) {
+        const float a = fabsf(z) * kInvSqrt2;
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
+        float q = fmaf(1.061405429f, t, -1.453152027f);
+        q = fmaf(q, t, 1.421413741f);
+        q = fmaf(q, t, -0.284496736f);
+        q = fmaf(q, t, 0.254829592f);
+        *e = __expf(-a * a);
+        const float tail = 0.5f * q * t * *e;
+        return z < 0.f ? tail : 1.f - tail;
+    } else {
+        *e = expf(-0.5f * z * z);
+        return 0.5f * erfcf(-z * kInvSqrt2);
+    }
+}
+
+template <bool FAST>
 __device__ __forceinline__ float act_value(float z, int act, float slope) {
     switch (act) {
         case kActRelu: return z <= 0.f ? 0.f : z;              // (NaN stays NaN)
         case kActLeaky: return z > 0.f ? z : z * slope;
-        case kActGelu: return z * (0.5f * erfcf(-z * kInvSqrt2));
-        case kActHardswish: return z * fminf(fmaxf(z + 3.f, 0.f), 6.f) / 6.f;
+        case kActGelu: {
+            float e;
+            return z * normal_cdf<FAST>(z, &e);
+        }
+        case kActHardswish: return z * fminf(fmaxf(z + 3.f, 0.f), 6.f) * (1.f / 6.f);
         default: return z;
     }
 }
 
+template <bool FAST>
 __device__ __forceinline__ float act_slope(float z, int act, float slope) {
     switch (act) {
         case kActRelu: return z <= 0.f ? 0.f : 1.f;
         case kActLeaky: return z > 0.f ? 1.f : slope;
         case kActGelu: {
-            const float c = fminf(fmaxf(z, -40.f), 40.f);      // beyond that z phi(z) is 0 and must not become inf * 0
-            return fmaf(c * kInvSqrt2Pi, expf(-0.5f * c * c), 0.5f * erfcf(-c * kInvSqrt2));
+            const float c = z > 40.f ? 40.f : (z < -40.f ? -40.f : z);      // beyond that z phi(z) is 0 and must not become inf * 0
+            float e;
+            const float cdf = normal_cdf<FAST>(c, &e);
+            return fmaf(c * kInvSqrt2Pi, e, cdf);
         }
-        case kActHardswish: return z <= -3.f ? 0.f : (z >= 3.f ? 1.f : (2.f * z + 3.f) / 6.f);
+        case kActHardswish: return z <= -3.f ? 0.f : (z >= 3.f ? 1.f : fmaf(2.f, z, 3.f) * (1.f / 6.f));
         default: return 1.f;
     }
 }
+
+// ---- element types ------------------------------------------------------------------------------------------------------------------
+// 16-byte pieces at any element-aligned address: the target takes unaligned global accesses, the type says so to the compiler
+struct __attribute__((packed, aligned(2))) Piece16 {
+    u32x4 v;
+};
+__device__ __forceinline__ u32x4 load16(const void* p) { return static_cast<const Piece16*>(p)->v; }
+__device__ __forceinline__ void store16(void* p, u32x4 v) { static_cast<Piece16*>(p)->v = v; }
+
+template <typename T> struct Num;
+template <> struct Num<float> {
+    static constexpr int E = 4;                   // elements of a 16-byte piece
+    static constexpr bool fast = false;
+    using Pre = float;
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned u = v[i];
+            f[i] = __builtin_bit_cast(float, u);
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[4]) {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(unsigned, f[i]);
+        return v;
+    }
+    static __device__ __forceinline__ float pre(float z) { return z; }
+    static __device__ __forceinline__ u32x4 pack_pre(const float (&f)[4]) { return pack(f); }
+    static __device__ __forceinline__ void unpack_pre(u32x4 v, float (&f)[4]) { unpack(v, f); }
+    // one k step: lane half h holds 4 consecutive k of its half, so A and B agree whatever k that is
+    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+        float x[4], y[4];
+        unpack(a, x);
+        unpack(b, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+        return c;
+    }
+};
 
 // What the backward needs of z: float32 for float32 rows, float16 for BOTH 16-bit types (the derivative saturates far inside float16's
 // range, and float16's 11 bits keep the saved value's rounding out of the gradients).  A positive z never becomes zero: the sign decides.
@@ -49,139 +118,741 @@ __device__ __forceinline__ f16_t pre_half(float z) {
     if (z > 0.f && h == (f16_t)0.f) h = __builtin_bit_cast(f16_t, (unsigned short)1);
     return h;
 }
-template <typename T> struct PreOf { using type = f16_t; };
-template <> struct PreOf<float> { using type = float; };
 
-template <typename T> __device__ __forceinline__ void store_pre(typename PreOf<T>::type* p, float z) { *p = pre_half(z); }
-template <> __device__ __forceinline__ void store_pre<float>(float* p, float z) { *p = z; }
+template <typename T> struct Num16 {
+    static constexpr int E = 8;
+    static constexpr bool fast = true;
+    using Pre = f16_t;
+    using V8 = __attribute__((ext_vector_type(8))) T;
+    using H8 = __attribute__((ext_vector_type(8))) f16_t;
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
+        const V8 t = __builtin_bit_cast(V8, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)t[i];
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+        V8 t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = (T)f[i];
+        return __builtin_bit_cast(u32x4, t);
+    }
+    static __device__ __forceinline__ f16_t pre(float z) { return pre_half(z); }
+    static __device__ __forceinline__ u32x4 pack_pre(const float (&f)[8]) {
+        H8 t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = pre_half(f[i]);
+        return __builtin_bit_cast(u32x4, t);
+    }
+    static __device__ __forceinline__ void unpack_pre(u32x4 v, float (&f)[8]) {
+        const H8 t = __builtin_bit_cast(H8, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)t[i];
+    }
+};
+template <> struct Num<bf16_t> : Num16<bf16_t> {
+    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+    }
+};
+template <> struct Num<f16_t> : Num16<f16_t> {
+    static __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
+    }
+};
 
-// ---- a plain tiled product, right for every shape and stride ------------------------------------------------------------------------
-// C[m, n] = sum_k A[m am + k ak] B[n bn + k bk]
+// elements [c, c + E) of a row of C columns (zeros behind its end); nothing outside the row is read
+template <typename T>
+__device__ __forceinline__ u32x4 load_piece(const T* row, long c, long C) {
+    constexpr int E = Num<T>::E;
+    if (c + E <= C) return load16(row + c);
+    T e[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) e[i] = c + i < C ? row[c + i] : (T)0.f;
+    return __builtin_bit_cast(u32x4, e);
+}
+
+// ---- rows times rows: out[m, n] = sum_k A[m, k] B[n, k], both k-contiguous ------------------------------------------------------------
+// The forward (A = x, B = w, with the epilogue) and the data gradient (A = dz, B = the transposed weight).
+//
+// A workgroup of WR x WC waves computes BM x BN outputs; a wave its (BM / WR) x (BN / WC) block out of 32 x 32 matrix-unit tiles, n in the
+// tile's rows: a lane ends up with four consecutive n of one m.  k advances in stages of CH 16-byte pieces per row (CH = 8: 64 sixteen-bit
+// or 32 float values), kept in LDS as [row][piece] with the piece index XORed by the row, so that the eight lanes that are served
+// together read eight different 16-byte columns.  In float32 a piece feeds four matrix instructions, in 16 bits one: the same addresses.
+//
+// DMA = 1: every row starts on 16 bytes and K is a whole number of pieces; stages go from memory to LDS without registers
+// (global_load_lds), NBUF - 1 stages ahead, one barrier a stage.  Rows behind the end are read from the last row (their outputs are not
+// stored), pieces behind K from sixteen zero bytes.
+// DMA = 0: any alignment and any K; a stage waits in registers while the previous one is multiplied.
+//
+// Epilogue: the sums go through LDS (the wave's own part of it, 32 rows at a time) so that a lane then holds E consecutive columns of a
+// row: bias, activation, residual and the stores are 16-byte accesses of whole lines.
+__device__ u32x4 g_zero_piece;      // stays zero
+
 struct Epilogue {
-    const void* bias;
+    const void* bias;      // per output column (all groups), or NULL
     int bias_f32;
     const void* residual;
     long ldr;
-    void* pre;             // dense rows of groups * N
+    void* pre;             // dense rows of ld_pre columns, or NULL
+    long ld_pre;
     int act;
     float slope;
 };
 
+template <int CH>
+__device__ __forceinline__ int swizzle(int row, int piece) {
+    if constexpr (CH == 8) return piece ^ (row & 7);
+    else return piece ^ ((row >> 1) & 3);
+}
+
+// LDS written by a wave is read by the same wave's other lanes behind this (its LDS instructions run in order)
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A 32-row strip of a wave's block into LDS: row = lane & 31, and the lane's four consecutive columns per 8 of each 32-column tile
+template <int SN, typename F>
+__device__ __forceinline__ void put_strip(float* strip, int ld, int lane, F value) {
+    const int r32 = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < SN; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(strip + r32 * ld + i * 32 + q * 8 + half * 4) =
+                make_float4(value(i, q * 4), value(i, q * 4 + 1), value(i, q * 4 + 2), value(i, q * 4 + 3));
+    wave_sync();
+}
+
+constexpr int kXcds = 8;
+
+// Workgroup -> (m tile, n tile).  The hardware deals workgroups out over the 8 XCDs in turn; each XCD gets a contiguous run of items, and
+// items walk 8 m tiles for every n tile, so that what runs together on an XCD shares panels of both operands in its L2.
+__device__ __forceinline__ bool tile_of(int block, int grid, int mt, int nt, int* m, int* n) {
+    const int per = grid / kXcds;
+    const long item = (long)(block % kXcds) * per + block / kXcds;
+    if (item >= (long)mt * nt) return false;
+    const int band = (int)(item / (8l * nt)), in = (int)(item % (8l * nt));
+    const int rows = min(8, mt - band * 8);
+    *m = band * 8 + in % rows;
+    *n = in / rows;
+    return true;
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void plain_gemm_kernel(const T* __restrict__ A, const T* __restrict__ B, T* __restrict__ C, long M,
-                                                         int N, long K, long am, long ak, long bn, long bk, long ldc, long ag, long bg,
-                                                         long cg, Epilogue e) {
-    __shared__ float As[16][65], Bs[16][65];
-    const int g = blockIdx.z;
-    const long m0 = (long)blockIdx.x * 64;
-    const int n0 = blockIdx.y * 64;
-    A += g * ag;
+__device__ __forceinline__ void finish_piece(float (&f)[Num<T>::E], const float (&bias)[Num<T>::E], T* out, const Epilogue& e, long m, long col,
+                                             int valid) {
+    constexpr int E = Num<T>::E;
+    using Pre = typename Num<T>::Pre;
+#pragma unroll
+    for (int i = 0; i < E; ++i) f[i] += bias[i];
+    if (e.pre) {
+        Pre* p = static_cast<Pre*>(e.pre) + m * e.ld_pre + col;
+        if (valid == E) store16(p, Num<T>::pack_pre(f));
+        else
+            for (int i = 0; i < E; ++i)
+                if (i < valid) p[i] = Num<T>::pre(f[i]);
+    }
+    if (e.act != kActNone) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = act_value<Num<T>::fast>(f[i], e.act, e.slope);
+    }
+    if (e.residual) {
+        float r[E];
+        Num<T>::unpack(load_piece(static_cast<const T*>(e.residual) + m * e.ldr + col, 0, valid), r);
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] += r[i];
+    }
+    if (valid == E) store16(out, Num<T>::pack(f));
+    else
+        for (int i = 0; i < E; ++i)
+            if (i < valid) out[i] = (T)f[i];
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias(float (&b)[Num<T>::E], const Epilogue& e, long col, int valid) {
+#pragma unroll
+    for (int i = 0; i < Num<T>::E; ++i) {
+        b[i] = 0.f;
+        if (e.bias && i < valid) b[i] = e.bias_f32 ? static_cast<const float*>(e.bias)[col + i] : (float)static_cast<const T*>(e.bias)[col + i];
+    }
+}
+
+template <typename T, int BM, int BN, int WR, int WC, int CH, int NBUF, int DMA>
+__global__ __launch_bounds__(64 * WR * WC, 2) void rows_gemm_kernel(
+    const T* __restrict__ A, const T* __restrict__ B, T* __restrict__ out, long M, int N, int K, long lda, long ldb, long ldo, long bg, int mt, int nt,
+    Epilogue e) {
+    constexpr int E = Num<T>::E, KE = CH * E, THREADS = 64 * WR * WC, WAVES = WR * WC;
+    constexpr int TM = BM / WR, TN = BN / WC, SM = TM / 32, SN = TN / 32;
+    constexpr int STAGE = (BM + BN) * CH;                        // pieces
+    extern __shared__ u32x4 smem[];
+    int mi, ni;
+    if (!tile_of(blockIdx.x, gridDim.x, mt, nt, &mi, &ni)) return;
+    const int g = blockIdx.y;
+    const long m0 = (long)mi * BM;
+    const int n0 = ni * BN;
+    A += (long)g * K;
     B += g * bg;
-    C += g * cg;
-    float acc[4][4] = {};
-    const int tm = threadIdx.x / 16, tn = threadIdx.x % 16;
-    for (long k0 = 0; k0 < K; k0 += 16) {
-        for (int i = threadIdx.x; i < 1024; i += 256) {
-            const int kk = i / 64, r = i % 64;
-            As[kk][r] = (m0 + r < M && k0 + kk < K) ? (float)A[(m0 + r) * am + (k0 + kk) * ak] : 0.f;
-            Bs[kk][r] = (n0 + r < N && k0 + kk < K) ? (float)B[(n0 + r) * bn + (k0 + kk) * bk] : 0.f;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WC, wn = wave % WC;
+    const int stages = (K + KE - 1) / KE;
+
+    f32x16 acc[SN][SM];
+#pragma unroll
+    for (int i = 0; i < SN; ++i)
+#pragma unroll
+        for (int j = 0; j < SM; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    auto multiply = [&](const u32x4* buf, int steps) __attribute__((always_inline)) {
+        const u32x4* as = buf + (wm * TM) * CH;
+        const u32x4* bs = buf + (BM + wn * TN) * CH;
+        const int r32 = lane & 31, half = lane >> 5;
+#pragma unroll
+        for (int ks = 0; ks < CH / 2; ++ks) {
+            if (ks < steps) {
+                u32x4 a[SM], b[SN];
+#pragma unroll
+                for (int j = 0; j < SM; ++j) a[j] = as[(j * 32 + r32) * CH + swizzle<CH>(r32, ks * 2 + half)];
+#pragma unroll
+                for (int i = 0; i < SN; ++i) b[i] = bs[(i * 32 + r32) * CH + swizzle<CH>(r32, ks * 2 + half)];
+#pragma unroll
+                for (int i = 0; i < SN; ++i)
+#pragma unroll
+                    for (int j = 0; j < SM; ++j) acc[i][j] = Num<T>::mma(b[i], a[j], acc[i][j]);
+            }
         }
+    };
+    const int last_steps = ((K - (stages - 1) * KE) + 2 * E - 1) / (2 * E);
+
+    if constexpr (DMA) {
+        // a wave's instruction fills 64 pieces: 64 / CH rows; A's BM rows first, then B's
+        constexpr int RPI = 64 / CH, INSTR = (BM + BN) / RPI / WAVES;
+        const char* src[INSTR];
+        int piece[INSTR];
+#pragma unroll
+        for (int i = 0; i < INSTR; ++i) {
+            const int row = (i * WAVES + wave) * RPI + lane / CH;          // INSTR x WAVES x RPI rows, A rows below BM
+            const int in = row < BM ? row : row - BM;
+            piece[i] = swizzle<CH>(in, lane % CH);
+            src[i] = row < BM ? reinterpret_cast<const char*>(A + min(m0 + in, M - 1) * lda)
+                              : reinterpret_cast<const char*>(B + (long)min(n0 + in, N - 1) * ldb);
+        }
+        const int pieces = K / E;
+        auto fetch = [&](int s) __attribute__((always_inline)) {
+            u32x4* buf = smem + (s % NBUF) * STAGE;
+            const bool whole = (s + 1) * CH <= pieces;
+#pragma unroll
+            for (int i = 0; i < INSTR; ++i) {
+                const int pc = s * CH + piece[i];
+                const char* from = src[i] + (long)pc * 16;
+                if (!whole && pc >= pieces) from = reinterpret_cast<const char*>(&g_zero_piece);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                                 (__attribute__((address_space(3))) void*)(buf + (i * WAVES + wave) * 64), 16, 0, 0);
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < NBUF - 1; ++s)
+            if (s < stages) fetch(s);
+        for (int s = 0; s < stages; ++s) {
+            // stage s has landed when at most the loads of the younger stages are still in flight (they return in order)
+            // and this wave's own reads of stage s - 1 are done
+            if (s + NBUF - 2 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF - 2) * INSTR) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();             // everybody's pieces are there, and nobody reads stage s - 1 any more
+            asm volatile("" ::: "memory");
+            if (s + NBUF - 1 < stages) fetch(s + NBUF - 1);
+            multiply(smem + (s % NBUF) * STAGE, s + 1 < stages ? CH / 2 : last_steps);
+        }
+    } else {
+        constexpr int PIECES = STAGE / THREADS;
+        u32x4 held[PIECES];
+        auto fetch = [&](int s, bool whole) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int f = i * THREADS + tid, row = f / CH, pc = f % CH;
+                const long k = (long)s * KE + pc * E;
+                const T* at = row < BM ? A + min(m0 + row, M - 1) * lda : B + (long)min(n0 + (row - BM), N - 1) * ldb;
+                held[i] = whole ? load16(at + k) : load_piece(at, k, K);
+            }
+        };
+        auto keep = [&](u32x4* buf) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int f = i * THREADS + tid, row = f / CH, pc = f % CH;
+                buf[row * CH + swizzle<CH>(row < BM ? row : row - BM, pc)] = held[i];
+            }
+        };
+        fetch(0, K >= KE);
+        keep(smem);
         __syncthreads();
-        for (int kk = 0; kk < 16; ++kk)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[kk][tm * 4 + i], Bs[kk][tn * 4 + j], acc[i][j]);
-        __syncthreads();
+        for (int s = 0; s < stages; ++s) {
+            if (s + 1 < stages) fetch(s + 1, (s + 2) * KE <= K);
+            multiply(smem + (s & 1) * STAGE, s + 1 < stages ? CH / 2 : last_steps);
+            if (s + 1 < stages) keep(smem + ((s + 1) & 1) * STAGE);      // read last in the multiplication before this one
+            __syncthreads();
+        }
     }
-    for (int i = 0; i < 4; ++i) {
-        const long m = m0 + tm * 4 + i;
-        if (m >= M) continue;
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + tn * 4 + j;
-            if (n >= N) continue;
-            float z = acc[i][j];
-            const long col = (long)g * N + n;
-            if (e.bias) z += e.bias_f32 ? static_cast<const float*>(e.bias)[col] : (float)static_cast<const T*>(e.bias)[col];
-            if (e.pre) store_pre<T>(static_cast<typename PreOf<T>::type*>(e.pre) + m * (long)(gridDim.z) * N + col, z);
-            z = act_value(z, e.act, e.slope);
-            if (e.residual) z += (float)static_cast<const T*>(e.residual)[m * e.ldr + col];
-            C[m * ldc + n] = (T)z;
+
+    // epilogue
+    constexpr int LD = TN + 4;                    // floats
+    static_assert(32 * LD * 4 * WAVES <= STAGE * 16 * NBUF, "a wave's strip has to fit into the stages' LDS");
+    float* strip = reinterpret_cast<float*>(smem) + wave * 32 * LD;
+    if constexpr (DMA) __syncthreads();
+    constexpr int LPR = TN / E, RPI = 64 / LPR;   // lanes per row, rows per pass
+    const int col = n0 + wn * TN + (lane % LPR) * E;
+    const int valid = min(E, N - col);
+    const long oc = (long)g * N + col;
+    float bias[E];
+    load_bias<T>(bias, e, oc, valid);
+#pragma unroll
+    for (int j = 0; j < SM; ++j) {
+        put_strip<SN>(strip, LD, lane, [&](int i, int r) { return acc[i][j][r]; });
+#pragma unroll
+        for (int r = 0; r < 32; r += RPI) {
+            const int row = r + lane / LPR;
+            const long m = m0 + wm * TM + j * 32 + row;
+            float f[E];
+#pragma unroll
+            for (int q = 0; q < E; q += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(strip + row * LD + (lane % LPR) * E + q);
+                f[q] = v.x, f[q + 1] = v.y, f[q + 2] = v.z, f[q + 3] = v.w;
+            }
+            if (m < M && valid > 0) finish_piece<T>(f, bias, out + m * ldo + oc, e, m, oc, valid);
         }
+        wave_sync();
     }
 }
 
-// dz = gy * act'(saved), dense rows; saved is z (kind 1) or, for the activations whose sign is z's, y itself (kind 2)
-template <typename T>
-__global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ gy, const void* __restrict__ saved, T* __restrict__ dz, long P,
-                                                       long C, long ldg, int kind, int act, float slope) {
-    const long total = P * C;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long p = i / C, c = i % C;
-        const float s = kind == 2 ? (float)static_cast<const T*>(saved)[i] : (float)static_cast<const typename PreOf<T>::type*>(saved)[i];
-        dz[i] = (T)((float)gy[p * ldg + c] * act_slope(s, act, slope));
+template <typename T, int BM, int BN, int WR, int WC, int CH, int NBUF, int DMA>
+void launch_rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
+                      hipStream_t s) {
+    const int mt = (int)cdiv64(M, BM), nt = cdiv(N, BN);
+    const size_t lds = (size_t)(BM + BN) * CH * 16 * NBUF;
+    auto* kernel = &rows_gemm_kernel<T, BM, BN, WR, WC, CH, NBUF, DMA>;
+    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    const int64_t items = (int64_t)mt * nt;
+    const dim3 grid((unsigned)(cdiv64(items, kXcds) * kXcds), (unsigned)groups);
+    hipLaunchKernelGGL((rows_gemm_kernel<T, BM, BN, WR, WC, CH, NBUF, DMA>), grid, dim3(64 * WR * WC), lds, s, A, B, out, M, N, K, lda, ldb, ldo, bg,
+                       mt, nt, e);
+}
+
+bool on16(const void* p, long ld, size_t size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (long)size % 16 == 0; }
+
+// ---- the weight gradient: out[n, k] = sum_p G[p, n] X[p, k], both reduced over their ROWS ------------------------------------------------
+// A stage is KP rows of BC columns of each operand, as they lie in memory.  16 bits: the matrix unit wants 8 consecutive p of one column per
+// lane, which ds_read_tr16_b64 delivers: the 16 lanes of a group name 4 rows x 16 columns (8 bytes each) and each receives one column's
+// four values.  The 64-byte granules of a row are XORed by the row so that the four rows fall on different banks.  float32: the
+// instruction takes one p per lane half, plain 4-byte reads.
+// k is put in the tile's rows, so a lane ends up with consecutive k and the epilogue above stores whole lines of the weight's layout.
+// p is split over blockIdx.z when there are few tiles: float32 partial blocks, added in a fixed order by split_sum_kernel.
+template <typename T, int BC>
+__device__ __forceinline__ int col_swizzle(int row, int piece) {
+    if constexpr (sizeof(T) == 4) return piece;
+    else if constexpr (BC == 64) return piece ^ (((row >> 1) & 1) << 2);
+    else return piece ^ ((row & 3) << 2);
+}
+
+template <typename T, int BC, int WR, int WC, int DMA>
+__global__ __launch_bounds__(64 * WR * WC, 2) void cols_gemm_kernel(const T* __restrict__ G, const T* __restrict__ X, T* __restrict__ out,
+                                                                    float* __restrict__ partial, long P, int N, int K, long ldg, long ldx, int nt,
+                                                                    int kt, long rows_per_split) {
+    constexpr int E = Num<T>::E, CP = BC / E, THREADS = 64 * WR * WC, WAVES = WR * WC, NBUF = 2;
+    constexpr int KP = sizeof(T) == 4 ? 32 : 64, HALF = KP * CP, STAGE = 2 * HALF;       // pieces; G's tile, then X's
+    constexpr int TM = BC / WR, TN = BC / WC, SM = TM / 32, SN = TN / 32;
+    extern __shared__ u32x4 smem[];
+    int ni, ki;
+    if (!tile_of(blockIdx.x, gridDim.x, nt, kt, &ni, &ki)) return;
+    const int g = blockIdx.y, n0 = ni * BC, k0 = ki * BC;
+    const long p_from = (long)blockIdx.z * rows_per_split, p_to = min(P, p_from + rows_per_split);
+    G += (long)g * N;
+    X += (long)g * K;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave / WC, wn = wave % WC;
+    const int stages = (int)((p_to - p_from + KP - 1) / KP);
+
+    f32x16 acc[SN][SM];
+#pragma unroll
+    for (int i = 0; i < SN; ++i)
+#pragma unroll
+        for (int j = 0; j < SM; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    auto multiply = [&](const u32x4* buf) __attribute__((always_inline)) {
+        if constexpr (sizeof(T) == 4) {
+            const float* gs = reinterpret_cast<const float*>(buf);
+            const float* xs = gs + KP * BC;
+            const int r32 = lane & 31, half = lane >> 5;
+#pragma unroll 8
+            for (int kk = 0; kk < KP / 2; ++kk) {
+                float a[SM], b[SN];
+#pragma unroll
+                for (int j = 0; j < SM; ++j) a[j] = gs[(kk * 2 + half) * BC + wm * TM + j * 32 + r32];
+#pragma unroll
+                for (int i = 0; i < SN; ++i) b[i] = xs[(kk * 2 + half) * BC + wn * TN + i * 32 + r32];
+#pragma unroll
+                for (int i = 0; i < SN; ++i)
+#pragma unroll
+                    for (int j = 0; j < SM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[i], a[j], acc[i][j], 0, 0, 0);
+            }
+        } else {
+            using S4 = __attribute__((ext_vector_type(4))) short;
+            auto read = [&](const u32x4* tile, int ks, int c0) __attribute__((always_inline)) {
+                const int row = ks * 16 + 8 * (lane >> 5) + ((lane >> 2) & 3), col = c0 + 16 * ((lane >> 4) & 1) + (lane & 3) * 4;
+                const char* at = reinterpret_cast<const char*>(tile) + (row * CP + col_swizzle<T, BC>(row, col / 8)) * 16 + (col & 4) * 2;
+                // four rows further: the same swizzle
+                const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)at);
+                const S4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)(at + 4 * CP * 16));
+                return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+#pragma unroll
+            for (int ks = 0; ks < KP / 16; ++ks) {
+                u32x4 a[SM], b[SN];
+#pragma unroll
+                for (int j = 0; j < SM; ++j) a[j] = read(buf, ks, wm * TM + j * 32);
+#pragma unroll
+                for (int i = 0; i < SN; ++i) b[i] = read(buf + HALF, ks, wn * TN + i * 32);
+#pragma unroll
+                for (int i = 0; i < SN; ++i)
+#pragma unroll
+                    for (int j = 0; j < SM; ++j) acc[i][j] = Num<T>::mma(b[i], a[j], acc[i][j]);
+            }
+        }
+    };
+
+    if constexpr (DMA) {
+        constexpr int INSTR = STAGE / 64 / WAVES;
+        auto fetch = [&](int s) __attribute__((always_inline)) {
+            u32x4* buf = smem + (s % NBUF) * STAGE;
+#pragma unroll
+            for (int i = 0; i < INSTR; ++i) {
+                const int q = (i * WAVES + wave) * 64 + lane, in = q < HALF ? q : q - HALF;
+                const int row = in / CP, piece = col_swizzle<T, BC>(row, in % CP);
+                const long p = p_from + (long)s * KP + row;
+                const int c = (q < HALF ? n0 : k0) + piece * E;
+                const char* from = reinterpret_cast<const char*>(&g_zero_piece);
+                if (p < p_to && c < (q < HALF ? N : K)) from = reinterpret_cast<const char*>(q < HALF ? G + p * ldg + c : X + p * ldx + c);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                                 (__attribute__((address_space(3))) void*)(buf + (i * WAVES + wave) * 64), 16, 0, 0);
+            }
+        };
+        if (stages > 0) fetch(0);
+        for (int s = 0; s < stages; ++s) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (s + 1 < stages) fetch(s + 1);
+            multiply(smem + (s % NBUF) * STAGE);
+        }
+        __syncthreads();
+    } else {
+        constexpr int PIECES = STAGE / THREADS;
+        u32x4 held[PIECES];
+        const bool cols_whole = n0 + BC <= N && k0 + BC <= K;
+        auto fetch = [&](int s) __attribute__((always_inline)) {
+            const bool whole = cols_whole && p_from + (long)(s + 1) * KP <= p_to;
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int q = i * THREADS + tid, in = q < HALF ? q : q - HALF;
+                const int row = in / CP, c = (q < HALF ? n0 : k0) + (in % CP) * E;
+                const long p = p_from + (long)s * KP + row;
+                const T* at = q < HALF ? G + p * ldg : X + p * ldx;
+                if (whole) held[i] = load16(at + c);
+                else {
+                    held[i] = u32x4{0, 0, 0, 0};
+                    if (p < p_to) held[i] = load_piece(at, c, q < HALF ? N : K);
+                }
+            }
+        };
+        auto keep = [&](u32x4* buf) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+                const int q = i * THREADS + tid, in = q < HALF ? q : q - HALF, row = in / CP;
+                buf[q - in + row * CP + col_swizzle<T, BC>(row, in % CP)] = held[i];
+            }
+        };
+        if (stages > 0) {
+            fetch(0);
+            keep(smem);
+        }
+        __syncthreads();
+        for (int s = 0; s < stages; ++s) {
+            if (s + 1 < stages) fetch(s + 1);
+            multiply(smem + (s & 1) * STAGE);
+            if (s + 1 < stages) keep(smem + ((s + 1) & 1) * STAGE);
+            __syncthreads();
+        }
+    }
+
+    constexpr int LD = TN + 4;
+    static_assert(32 * LD * 4 * WAVES <= STAGE * 16 * NBUF, "a wave's strip has to fit into the stages' LDS");
+    float* strip = reinterpret_cast<float*>(smem) + wave * 32 * LD;
+    const long block = (long)g * N * K;
+    if (partial) partial += ((long)blockIdx.z * gridDim.y) * N * K + block;
+    else out += block;
+#pragma unroll
+    for (int j = 0; j < SM; ++j) {
+        put_strip<SN>(strip, LD, lane, [&](int i, int r) { return acc[i][j][r]; });
+        constexpr int LPR = TN / 4, RPI = 64 / LPR;
+        const int k = k0 + wn * TN + (lane % LPR) * 4;
+#pragma unroll
+        for (int r = 0; r < 32; r += RPI) {
+            const int row = r + lane / LPR, n = n0 + wm * TM + j * 32 + row;
+            const float4 v = *reinterpret_cast<const float4*>(strip + row * LD + (lane % LPR) * 4);
+            const float f[4] = {v.x, v.y, v.z, v.w};
+            if (n < N) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (k + q < K) {
+                        if (partial) partial[(long)n * K + k + q] = f[q];
+                        else out[(long)n * K + k + q] = (T)f[q];
+                    }
+            }
+        }
+        wave_sync();
     }
 }
 
+// out[i] = sum over splits of partial[split][i], in a fixed order: `parts` threads take a contiguous run of the splits each (one when there
+// are few: then every thread reads whole lines), and their sums are added in order
 template <typename T>
-__global__ __launch_bounds__(256) void column_sum_kernel(const T* __restrict__ gy, const void* __restrict__ saved, void* __restrict__ gb,
-                                                         int gb_f32, long P, long C, long ldg, int kind, int act, float slope) {
-    __shared__ float part[4][64];
-    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int w = threadIdx.x >> 6;
-    float acc = 0.f;
-    if (c < C)
-        for (long p = w; p < P; p += 4) {
-            float v = (float)gy[p * ldg + c];
-            if (kind == 1) v *= act_slope((float)static_cast<const typename PreOf<T>::type*>(saved)[p * C + c], act, slope);
-            if (kind == 2) v *= act_slope((float)static_cast<const T*>(saved)[p * C + c], act, slope);
-            acc += v;
-        }
-    part[w][threadIdx.x & 63] = acc;
+__global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict__ partial, void* __restrict__ out, int out_f32, long n, int splits,
+                                                        int parts) {
+    __shared__ float sums[256];
+    const int per = 256 / parts, part = threadIdx.x / per;
+    const long i = (long)blockIdx.x * per + threadIdx.x % per;
+    const int from = (int)((long)splits * part / parts), to = (int)((long)splits * (part + 1) / parts);
+    float t = 0.f;
+    if (i < n) {
+#pragma unroll 8
+        for (int s = from; s < to; ++s) t += partial[s * n + i];
+    }
+    sums[threadIdx.x] = t;
     __syncthreads();
-    if (w == 0 && c < C) {
-        const float t = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
-        if (gb_f32) static_cast<float*>(gb)[c] = t;
-        else static_cast<T*>(gb)[c] = (T)t;
+    if (part != 0 || i >= n) return;
+    for (int q = 1; q < parts; ++q) t += sums[q * per + threadIdx.x];
+    if (out_f32) static_cast<float*>(out)[i] = t;
+    else static_cast<T*>(out)[i] = (T)t;
+}
+
+// ---- the activation's gradient and the column sums ------------------------------------------------------------------------------------
+// dz = gy act'(saved) as dense rows of ld_dz columns (a multiple of 16 bytes, so that both products fetch it without registers; the columns
+// behind C are zeros), and per-workgroup column sums of the unrounded dz.  A workgroup holds `lanes` 16-byte pieces of a row and 256 / lanes
+// rows at a time; blockIdx.x walks the pieces, blockIdx.y the rows.  Reads gy and the saved tensor, writes dz: HBM-bound.
+// KIND 0: no activation (only the sums), 1: saved is z, 2: saved is y and only its sign matters
+template <typename T, int KIND>
+__global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ gy, const void* __restrict__ saved, T* __restrict__ dz,
+                                                       float* __restrict__ sums, long P, long C, long ldg, long ld_dz, int lanes, long rows_per_block,
+                                                       int act, float slope) {
+    constexpr int E = Num<T>::E;
+    __shared__ float part[256][E + 1];
+    const int rows = 256 / lanes, r = threadIdx.x / lanes, piece = blockIdx.x * lanes + threadIdx.x % lanes;
+    const long c = (long)piece * E;
+    const long from = blockIdx.y * rows_per_block, to = min(P, from + rows_per_block);
+    float acc[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = 0.f;
+    if (r < rows && c < ld_dz) {
+        const int valid = (int)max(0l, min((long)E, C - c));
+#pragma unroll 4
+        for (long p = from + r; p < to; p += rows) {
+            float f[E];
+            Num<T>::unpack(load_piece(gy + p * ldg + c, 0, valid), f);
+            if constexpr (KIND == 1) {
+                float s[E];
+                Num<T>::unpack_pre(load_piece(static_cast<const typename Num<T>::Pre*>(saved) + p * C + c, 0, valid), s);
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[i] *= act_slope<Num<T>::fast>(s[i], act, slope);
+            }
+            if constexpr (KIND == 2) {
+                float s[E];
+                Num<T>::unpack(load_piece(static_cast<const T*>(saved) + p * C + c, 0, valid), s);
+#pragma unroll
+                for (int i = 0; i < E; ++i) f[i] *= act == kActRelu ? (s[i] <= 0.f ? 0.f : 1.f) : (s[i] > 0.f ? 1.f : slope);
+            }
+            if constexpr (KIND != 0) {
+                if (dz) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+                        if (i >= valid) f[i] = 0.f;
+                    store16(dz + p * ld_dz + c, Num<T>::pack(f));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[i] += f[i];
+        }
+    }
+    if (!sums) return;
+#pragma unroll
+    for (int i = 0; i < E; ++i) part[threadIdx.x][i] = acc[i];
+    __syncthreads();
+    if (r == 0 && c < C) {
+        for (int i = 0; i < E && c + i < C; ++i) {
+            float t = 0.f;
+            for (int q = 0; q < rows; ++q) t += part[q * lanes + threadIdx.x][i];
+            sums[blockIdx.y * C + c + i] = t;
+        }
     }
 }
 
+// w (groups * N, K) -> wt (groups * K, ldt >= N), columns behind N zero: the data gradient's second operand with n contiguous
+template <typename T>
+__global__ __launch_bounds__(256) void transpose_weight_kernel(const T* __restrict__ w, T* __restrict__ wt, int N, int K, int ldt) {
+    __shared__ T tile[64][66];
+    const int n0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
+    w += (long)blockIdx.z * N * K;
+    wt += (long)blockIdx.z * K * ldt;
+    for (int i = threadIdx.x; i < 4096; i += 256) {
+        const int n = n0 + i / 64, k = k0 + i % 64;
+        tile[i / 64][i % 64] = n < N && k < K ? w[(long)n * K + k] : (T)0.f;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 4096; i += 256) {
+        const int k = k0 + i / 64, n = n0 + i % 64;
+        if (k < K && n < ldt) wt[(long)k * ldt + n] = tile[i % 64][i / 64];
+    }
+}
+
+// ---- plans ---------------------------------------------------------------------------------------------------------------------------
 size_t elem_bytes(int dtype) { return dtype == 0 ? 4 : 2; }
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 template <typename T>
-int launch_fwd(const T* x, const T* w, T* y, int64_t P, int N, int K, int groups, int64_t ldx, int64_t ldy, const Epilogue& e,
+void rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
                hipStream_t s) {
-    const dim3 grid((unsigned)cdiv64(P, 64), (unsigned)cdiv(N, 64), (unsigned)groups);
-    hipLaunchKernelGGL(plain_gemm_kernel<T>, grid, dim3(256), 0, s, x, w, y, (long)P, N, (long)K, (long)ldx, 1l, (long)K, 1l, (long)ldy,
-                       (long)K, (long)N * K, (long)N, e);
+    constexpr size_t S = sizeof(T);
+    const bool dma = on16(A, lda, S) && on16(B, ldb, S) && (long)K * S % 16 == 0 && bg * (long)S % 16 == 0;
+    const int64_t big = cdiv64(M, 128) * cdiv(N, 128) * groups;
+    if (dma && big >= 256) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else if (dma) launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else if (big >= 256) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+}
+
+// The weight gradient's tiles and split: 128-column tiles, 64 where a side is that small; p in as many parts as give every CU two
+// workgroups, each at least eight stages long.
+struct ColsPlan {
+    int bc, nt, kt, splits;
+    long rows_per_split;
+};
+ColsPlan plan_cols(int64_t P, int N, int K, int groups, int dtype) {
+    ColsPlan p;
+    p.bc = N > 64 && K > 64 ? 128 : 64;
+    p.nt = cdiv(N, p.bc);
+    p.kt = cdiv(K, p.bc);
+    const int64_t tiles = (int64_t)p.nt * p.kt * groups, kp = dtype == 0 ? 32 : 64;
+    int64_t splits = cdiv64(512, tiles), most = cdiv64(P, 4 * kp);
+    if (splits > most) splits = most;
+    if (splits > 512) splits = 512;
+    p.rows_per_split = cdiv64(cdiv64(P, splits), kp) * kp;
+    p.splits = (int)cdiv64(P, p.rows_per_split);
+    return p;
+}
+
+template <typename T, int BC, int DMA>
+void launch_cols_gemm(const T* G, const T* X, T* out, float* partial, long P, int N, int K, int groups, long ldg, long ldx, const ColsPlan& p,
+                      hipStream_t s) {
+    constexpr int KP = sizeof(T) == 4 ? 32 : 64;
+    const size_t lds = (size_t)2 * 2 * KP * BC * sizeof(T);
+    const dim3 grid((unsigned)(cdiv64((int64_t)p.nt * p.kt, kXcds) * kXcds), (unsigned)groups, (unsigned)p.splits);
+    hipLaunchKernelGGL((cols_gemm_kernel<T, BC, 2, 2, DMA>), grid, dim3(256), lds, s, G, X, out, p.splits > 1 ? partial : nullptr, P, N, K, ldg,
+                       ldx, p.nt, p.kt, p.rows_per_split);
+}
+
+template <typename T>
+void split_sum(const float* partial, void* out, int out_f32, long n, int splits, hipStream_t s) {
+    const int parts = splits >= 64 ? 16 : (splits >= 16 && n < 65536 ? 4 : 1);
+    hipLaunchKernelGGL(split_sum_kernel<T>, dim3((unsigned)cdiv64(n, 256 / parts)), dim3(256), 0, s, partial, out, out_f32, n, splits, parts);
+}
+
+// `padded`: G's rows are followed by zeros up to whole pieces
+template <typename T>
+void cols_gemm(const T* G, const T* X, T* out, float* partial, long P, int N, int K, int groups, long ldg, long ldx, bool padded, int dtype,
+               hipStream_t s) {
+    constexpr size_t S = sizeof(T);
+    const ColsPlan p = plan_cols(P, N, K, groups, dtype);
+    const bool dma = on16(G, ldg, S) && on16(X, ldx, S) && (long)K * S % 16 == 0 && ((long)N * S % 16 == 0 || (padded && groups == 1));
+    if (p.bc == 128 && dma) launch_cols_gemm<T, 128, 1>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    else if (p.bc == 128) launch_cols_gemm<T, 128, 0>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    else if (dma) launch_cols_gemm<T, 64, 1>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    else launch_cols_gemm<T, 64, 0>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    if (p.splits > 1) split_sum<T>(partial, out, 0, (long)groups * N * K, p.splits, s);
+}
+
+// Workspace of a backward call: [dz][transposed weight][column sums][split blocks]
+struct BwdPlan {
+    int64_t ld_dz;
+    int ldt, lanes, col_blocks, row_blocks;
+    int64_t rows_per_block;
+    size_t dz, wt, sums, split, total;
+    ColsPlan cols;
+};
+BwdPlan plan_bwd(int64_t P, int N, int K, int groups, int dtype, int act, bool want_gx, bool want_gw, bool want_gb) {
+    BwdPlan b{};
+    const size_t S = elem_bytes(dtype);
+    const int E = dtype == 0 ? 4 : 8;
+    const int64_t C = (int64_t)groups * N;
+    b.ld_dz = cdiv64(C, E) * E;
+    b.ldt = cdiv(N, E) * E;
+    const int64_t pieces = b.ld_dz / E;
+    b.col_blocks = (int)cdiv64(pieces, 256);
+    b.lanes = (int)cdiv64(pieces, b.col_blocks);
+    const int rows = 256 / b.lanes;                       // rows a workgroup holds at a time; at least 8 of them each, about 1024 workgroups
+    int64_t blocks = cdiv64(1024, b.col_blocks), most = cdiv64(P, 8 * rows);
+    if (blocks > most) blocks = most;
+    b.rows_per_block = cdiv64(P, blocks);
+    b.row_blocks = (int)cdiv64(P, b.rows_per_block);
+    b.dz = act != kActNone && (want_gx || want_gw) ? align256((size_t)P * b.ld_dz * S) : 0;
+    b.wt = want_gx ? align256((size_t)groups * K * b.ldt * S) : 0;
+    b.sums = want_gb ? align256((size_t)b.row_blocks * C * 4) : 0;
+    b.cols = plan_cols(P, N, K, groups, dtype);
+    b.split = want_gw && b.cols.splits > 1 ? (size_t)b.cols.splits * groups * N * K * 4 : 0;
+    b.total = b.dz + b.wt + b.sums + b.split;
+    return b;
+}
+
+template <typename T>
+int launch_fwd(const T* x, const T* w, T* y, int64_t P, int N, int K, int groups, int64_t ldx, int64_t ldy, const Epilogue& e, hipStream_t s) {
+    rows_gemm<T>(x, w, y, P, N, K, groups, ldx, K, ldy, (long)N * K, e, s);
     return check_launch("linear_act_fwd");
 }
 
 template <typename T>
-int launch_bwd(const T* gy, const T* x, const T* w, const void* saved, int kind, T* gx, T* gw, void* gb, int gb_f32, T* dz, int64_t P,
-               int N, int K, int groups, int64_t ldg, int64_t ldx, int act, float slope, hipStream_t s) {
-    const long C = (long)groups * N;
-    const Epilogue none{};
-    if (gb)
-        hipLaunchKernelGGL(column_sum_kernel<T>, dim3((unsigned)cdiv64(C, 64)), dim3(256), 0, s, gy, saved, gb, gb_f32, (long)P, C, (long)ldg,
-                           kind, act, slope);
-    if (kind && (gx || gw)) {
-        const int64_t blocks = cdiv64(P * C, 256);
-        hipLaunchKernelGGL(act_grad_kernel<T>, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, gy, saved, dz, (long)P, C,
-                           (long)ldg, kind, act, slope);
-        gy = dz;
-        ldg = C;
+int launch_bwd(const T* gy, const T* x, const T* w, const void* saved, int kind, T* gx, T* gw, void* gb, int gb_f32, char* ws, int64_t P, int N,
+               int K, int groups, int64_t ldg, int64_t ldx, int dtype, int act, float slope, hipStream_t s) {
+    const BwdPlan b = plan_bwd(P, N, K, groups, dtype, act, gx != nullptr, gw != nullptr, gb != nullptr);
+    const int64_t C = (int64_t)groups * N;
+    T* dz = b.dz ? reinterpret_cast<T*>(ws) : nullptr;
+    T* wt = reinterpret_cast<T*>(ws + b.dz);
+    float* sums = gb ? reinterpret_cast<float*>(ws + b.dz + b.wt) : nullptr;
+    float* split = reinterpret_cast<float*>(ws + b.dz + b.wt + b.sums);
+    if (dz || sums) {
+        const dim3 grid((unsigned)b.col_blocks, (unsigned)b.row_blocks);
+        auto* kernel = kind == 0 ? &act_grad_kernel<T, 0> : (kind == 1 ? &act_grad_kernel<T, 1> : &act_grad_kernel<T, 2>);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, gy, saved, dz, sums, (long)P, (long)C, (long)ldg, (long)b.ld_dz, b.lanes,
+                           (long)b.rows_per_block, act, slope);
+        if (sums) split_sum<T>(sums, gb, gb_f32, C, b.row_blocks, s);
     }
-    if (gx)
-        hipLaunchKernelGGL(plain_gemm_kernel<T>, dim3((unsigned)cdiv64(P, 64), (unsigned)cdiv(K, 64), (unsigned)groups), dim3(256), 0, s, gy,
-                           w, gx, (long)P, K, (long)N, (long)ldg, 1l, 1l, (long)K, (long)groups * K, (long)N, (long)N * K, (long)K, none);
-    if (gw)
-        hipLaunchKernelGGL(plain_gemm_kernel<T>, dim3((unsigned)cdiv(N, 64), (unsigned)cdiv(K, 64), (unsigned)groups), dim3(256), 0, s, gy, x,
-                           gw, (long)N, K, (long)P, 1l, (long)ldg, 1l, (long)ldx, (long)K, (long)N, (long)K, (long)N * K, none);
+    const bool padded = dz != nullptr;
+    if (padded) {
+        gy = dz;
+        ldg = b.ld_dz;
+    }
+    if (gx) {
+        const Epilogue none{};
+        hipLaunchKernelGGL(transpose_weight_kernel<T>, dim3(cdiv(b.ldt, 64), cdiv(K, 64), groups), dim3(256), 0, s, w, wt, N, K, b.ldt);
+        // the zeros behind N in dz and in wt's rows are multiplied along: whole pieces
+        rows_gemm<T>(gy, wt, gx, P, K, padded && groups == 1 ? b.ldt : N, groups, ldg, b.ldt, (long)groups * K, (long)K * b.ldt, none, s);
+    }
+    if (gw) cols_gemm<T>(gy, x, gw, split, P, N, K, groups, ldg, ldx, padded, dtype, s);
     return check_launch("linear_act_bwd");
 }
 
 int check_sizes(const char* who, int64_t P, int N, int K, int groups, int dtype, int act) {
-    NEXTOU_REQUIRE(P > 0 && P <= (1ll << 36) && N > 0 && K > 0 && groups > 0 && groups <= 65535 && (int64_t)groups * N <= (1ll << 22) &&
-                       (int64_t)groups * K <= (1ll << 22),
+    NEXTOU_REQUIRE(P > 0 && P <= (1ll << 36) && N > 0 && K > 0 && groups > 0 && groups <= 65535 && (int64_t)groups * N <= (1ll << 21) &&
+                       (int64_t)groups * K <= (1ll << 21) && cdiv64(P, 64) * cdiv(N > K ? N : K, 64) < (1ll << 31),
                    "%s: bad sizes (P %lld, N %d, K %d, groups %d)", who, (long long)P, N, K, groups);
     NEXTOU_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d", who, dtype);
     NEXTOU_REQUIRE(act >= 0 && act <= 4, "%s: activation %d", who, act);
@@ -210,7 +881,7 @@ extern "C" int nextou_linear_act_fwd(const void* x, const void* w, const void* b
     size_t need = 0;
     nextou_linear_act_fwd_workspace(P, N, K, groups, dtype, &need);
     if (workspace_bytes < need) return fail(NEXTOU_ENOSPACE, "linear_act_fwd: workspace %zu < %zu bytes", workspace_bytes, need);
-    const Epilogue e{bias, bias_f32, residual, (long)ldr, pre, act, slope};
+    const Epilogue e{bias, bias_f32, residual, (long)ldr, pre, (long)groups * N, act, slope};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case 0: return launch_fwd<float>((const float*)x, (const float*)w, (float*)y, P, N, K, groups, ldx, ldy, e, s);
@@ -223,7 +894,7 @@ extern "C" int nextou_linear_act_bwd_workspace(int64_t P, int N, int K, int grou
                                                size_t* bytes) {
     if (int e = check_sizes("linear_act_bwd_workspace", P, N, K, groups, dtype, act)) return e;
     NEXTOU_REQUIRE(bytes, "linear_act_bwd_workspace: null pointer");
-    *bytes = act != kActNone && (want_gx || want_gw) ? (size_t)P * groups * N * elem_bytes(dtype) : 0;
+    *bytes = plan_bwd(P, N, K, groups, dtype, act, want_gx != 0, want_gw != 0, want_gb != 0).total;
     return 0;
 }
 
@@ -245,12 +916,12 @@ extern "C" int nextou_linear_act_bwd(const void* gy, const void* x, const void* 
     switch (dtype) {
         case 0:
             return launch_bwd<float>((const float*)gy, (const float*)x, (const float*)w, saved, saved_kind, (float*)gx, (float*)gw, gb, gb_f32,
-                                     (float*)workspace, P, N, K, groups, ldg, ldx, act, slope, s);
+                                     (char*)workspace, P, N, K, groups, ldg, ldx, dtype, act, slope, s);
         case 1:
             return launch_bwd<bf16_t>((const bf16_t*)gy, (const bf16_t*)x, (const bf16_t*)w, saved, saved_kind, (bf16_t*)gx, (bf16_t*)gw, gb,
-                                      gb_f32, (bf16_t*)workspace, P, N, K, groups, ldg, ldx, act, slope, s);
+                                      gb_f32, (char*)workspace, P, N, K, groups, ldg, ldx, dtype, act, slope, s);
         default:
             return launch_bwd<f16_t>((const f16_t*)gy, (const f16_t*)x, (const f16_t*)w, saved, saved_kind, (f16_t*)gx, (f16_t*)gw, gb, gb_f32,
-                                     (f16_t*)workspace, P, N, K, groups, ldg, ldx, act, slope, s);
+                                     (char*)workspace, P, N, K, groups, ldg, ldx, dtype, act, slope, s);
     }
 }
