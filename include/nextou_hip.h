@@ -605,12 +605,11 @@ int nextou_stem_bwd(const float* x, const float* gy, const uint32_t* act_mask, c
  *   gb = sum_p dz; any of gx (dense), gw (dense, like w), gb (float32 when gb_f32, else the rows' type) may be NULL.  saved_kind: 0 none
  *   (act 0), 1 `saved` is the forward's pre, 2 `saved` is the forward's y, dense (relu, leaky relu with slope >= 0 and no residual: its sign is z's).
  *   Sums over points in a fixed order: bit-reproducible.
- * workspace: the matching _workspace call's bytes, contents irrelevant; one per call in flight.
+ * workspace (backward): nextou_linear_act_bwd_workspace's bytes, contents irrelevant; one per call in flight.
  * ---------------------------------------------------------------------------------------- */
-int nextou_linear_act_fwd_workspace(int64_t P, int N, int K, int groups, int dtype, size_t* bytes);
-int nextou_linear_act_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre, void* workspace,
-                          size_t workspace_bytes, int64_t P, int N, int K, int groups, int64_t ldx, int64_t ldr, int64_t ldy, int dtype,
-                          int bias_f32, int act, float slope, nextou_stream_t stream);
+int nextou_linear_act_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre, int64_t P,
+                          int N, int K, int groups, int64_t ldx, int64_t ldr, int64_t ldy, int dtype, int bias_f32, int act, float slope,
+                          nextou_stream_t stream);
 int nextou_linear_act_bwd_workspace(int64_t P, int N, int K, int groups, int dtype, int act, int want_gx, int want_gw, int want_gb,
                                     size_t* bytes);
 int nextou_linear_act_bwd(const void* gy, const void* x, const void* w, const void* saved, int saved_kind, void* gx, void* gw, void* gb,

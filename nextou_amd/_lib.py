@@ -130,9 +130,8 @@ _SIGNATURES = {
     "nextou_stem_workspace_bytes": (c_size_t, [c_int] * 5),
     "nextou_stem_fwd": (c_int, [c_void_p] * 13 + [c_size_t] + [c_int] * 7 + [c_float, c_float, c_float, c_void_p]),
     "nextou_stem_bwd": (c_int, [c_void_p] * 12 + [c_size_t] + [c_int] * 6 + [c_float, c_void_p]),
-    "nextou_linear_act_fwd_workspace": (c_int, [c_int64, c_int, c_int, c_int, c_int, ctypes.POINTER(c_size_t)]),
-    "nextou_linear_act_fwd": (c_int, [c_void_p] * 7 + [c_size_t, c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_int,
-                                      c_float, c_void_p]),
+    "nextou_linear_act_fwd": (c_int, [c_void_p] * 6 + [c_int64, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_float,
+                                      c_void_p]),
     "nextou_linear_act_bwd_workspace": (c_int, [c_int64] + [c_int] * 8 + [ctypes.POINTER(c_size_t)]),
     "nextou_linear_act_bwd": (c_int, [c_void_p] * 4 + [c_int] + [c_void_p] * 4 + [c_size_t, c_int64, c_int, c_int, c_int, c_int64, c_int64,
                                                                                 c_int, c_int, c_int, c_float, c_void_p]),

@@ -40,17 +40,29 @@ __device__ __forceinline__ float normal_cdf(float z, float* e) {
     }
 }
 
-template <bool FAST>
-__device__ __forceinline__ float act_value(float z, int act, float slope) {
-    switch (act) {
-        case kActRelu: return z <= 0.f ? 0.f : z;              // (NaN stays NaN)
-        case kActLeaky: return z > 0.f ? z : z * slope;
-        case kActGelu: {
-            float e;
-            return z * normal_cdf<FAST>(z, &e);
+// (one branch for a piece, not one for every element)
+template <bool FAST, int E>
+__device__ __forceinline__ void activate(float (&f)[E], int act, float slope) {
+    if (act == kActRelu) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = f[i] <= 0.f ? 0.f : f[i];             // (NaN stays NaN)
+    } else if (act == kActLeaky) {
+        if (slope >= 0.f && slope <= 1.f) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] = fmaxf(f[i], f[i] * slope);
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] = f[i] > 0.f ? f[i] : f[i] * slope;
         }
-        case kActHardswish: return z * fminf(fmaxf(z + 3.f, 0.f), 6.f) * (1.f / 6.f);
-        default: return z;
+    } else if (act == kActGelu) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            float e;
+            f[i] *= normal_cdf<FAST>(f[i], &e);
+        }
+    } else if (act == kActHardswish) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) f[i] = f[i] * fminf(fmaxf(f[i] + 3.f, 0.f), 6.f) * (1.f / 6.f);
     }
 }
 
@@ -171,6 +183,28 @@ __device__ __forceinline__ u32x4 load_piece(const T* row, long c, long C) {
     return __builtin_bit_cast(u32x4, e);
 }
 
+// The same without a branch around the load, so that many can be in flight (C >= E): the last whole piece of the row is fetched where the
+// wanted one would pass its end, and tail_fixed() moves the wanted elements down when the value is used.
+template <typename T>
+__device__ __forceinline__ u32x4 load_tail(const T* row, long c, long C) {
+    return load16(row + min(c, C - Num<T>::E));
+}
+template <typename T>
+__device__ __forceinline__ u32x4 tail_fixed(u32x4 v, long c, long C) {
+    constexpr int E = Num<T>::E, BITS = 8 * sizeof(T);
+    const int over = (int)max(0l, min((long)E, c + E - C)) * BITS;      // bits to drop: 0 ... 128
+    unsigned long long lo = v[0] | (unsigned long long)v[1] << 32, hi = v[2] | (unsigned long long)v[3] << 32;
+    if (over >= 64) {
+        lo = hi;
+        hi = 0;
+    }
+    const int sh = over & 63;
+    lo = sh ? lo >> sh | hi << (64 - sh) : lo;
+    hi >>= sh;
+    if (over == 128) lo = 0;
+    return u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
+}
+
 // ---- rows times rows: out[m, n] = sum_k A[m, k] B[n, k], both k-contiguous ------------------------------------------------------------
 // The forward (A = x, B = w, with the epilogue) and the data gradient (A = dz, B = the transposed weight).
 //
@@ -193,8 +227,7 @@ struct Epilogue {
     int bias_f32;
     const void* residual;
     long ldr;
-    void* pre;             // dense rows of ld_pre columns, or NULL
-    long ld_pre;
+    void* pre;             // dense rows, or NULL
     int act;
     float slope;
 };
@@ -239,42 +272,63 @@ __device__ __forceinline__ bool tile_of(int block, int grid, int mt, int nt, int
     return true;
 }
 
+// One output row of the epilogue: where its residual, its z and the row itself begin, and how many columns there are in all
 template <typename T>
-__device__ __forceinline__ void finish_piece(float (&f)[Num<T>::E], const float (&bias)[Num<T>::E], T* out, const Epilogue& e, long m, long col,
-                                             int valid) {
+struct OutRow {
+    const T* residual;
+    typename Num<T>::Pre* pre;
+    T* out;
+    int C;
+    __device__ __forceinline__ OutRow(const Epilogue& e, T* first, long ldo, long m, int C) : C(C) {
+        residual = e.residual ? static_cast<const T*>(e.residual) + m * e.ldr : nullptr;
+        pre = e.pre ? static_cast<typename Num<T>::Pre*>(e.pre) + m * C : nullptr;
+        out = first + m * ldo;
+    }
+    __device__ __forceinline__ u32x4 fetch(int col) const { return load_tail(residual, col, C); }       // C >= E
+};
+
+template <typename T>
+__device__ __forceinline__ void finish_piece(float (&f)[Num<T>::E], u32x4 residual, const OutRow<T>& row, int col, int valid, int act, float slope) {
     constexpr int E = Num<T>::E;
-    using Pre = typename Num<T>::Pre;
-#pragma unroll
-    for (int i = 0; i < E; ++i) f[i] += bias[i];
-    if (e.pre) {
-        Pre* p = static_cast<Pre*>(e.pre) + m * e.ld_pre + col;
+    if (row.pre) {
+        typename Num<T>::Pre* p = row.pre + col;
         if (valid == E) store16(p, Num<T>::pack_pre(f));
         else
             for (int i = 0; i < E; ++i)
                 if (i < valid) p[i] = Num<T>::pre(f[i]);
     }
-    if (e.act != kActNone) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = act_value<Num<T>::fast>(f[i], e.act, e.slope);
-    }
-    if (e.residual) {
+    activate<Num<T>::fast>(f, act, slope);
+    if (row.residual) {
         float r[E];
-        Num<T>::unpack(load_piece(static_cast<const T*>(e.residual) + m * e.ldr + col, 0, valid), r);
+        if (col + E <= row.C) Num<T>::unpack(residual, r);
+        else if (row.C >= E) Num<T>::unpack(tail_fixed<T>(residual, col, row.C), r);
+        else
+            for (int i = 0; i < E; ++i) r[i] = i < valid ? (float)row.residual[col + i] : 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) f[i] += r[i];
     }
+    T* out = row.out + col;
     if (valid == E) store16(out, Num<T>::pack(f));
     else
         for (int i = 0; i < E; ++i)
             if (i < valid) out[i] = (T)f[i];
 }
 
+// bias of columns col ... col + E - 1 of C (no branch around a load: eight of them in a row would cost eight memory latencies)
 template <typename T>
-__device__ __forceinline__ void load_bias(float (&b)[Num<T>::E], const Epilogue& e, long col, int valid) {
+__device__ __forceinline__ void load_bias(float (&b)[Num<T>::E], const Epilogue& e, int col, int C) {
+    constexpr int E = Num<T>::E;
 #pragma unroll
-    for (int i = 0; i < Num<T>::E; ++i) {
-        b[i] = 0.f;
-        if (e.bias && i < valid) b[i] = e.bias_f32 ? static_cast<const float*>(e.bias)[col + i] : (float)static_cast<const T*>(e.bias)[col + i];
+    for (int i = 0; i < E; ++i) b[i] = 0.f;
+    if (!e.bias) return;
+    if (e.bias_f32) {
+        const float* p = static_cast<const float*>(e.bias);
+#pragma unroll
+        for (int i = 0; i < E; ++i) b[i] = p[min(col + i, C - 1)];
+    } else {
+        const T* p = static_cast<const T*>(e.bias);
+#pragma unroll
+        for (int i = 0; i < E; ++i) b[i] = (float)p[min(col + i, C - 1)];
     }
 }
 
@@ -368,29 +422,32 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void rows_gemm_kernel(
     } else {
         constexpr int PIECES = STAGE / THREADS;
         u32x4 held[PIECES];
-        auto fetch = [&](int s, bool whole) __attribute__((always_inline)) {
+        const int pc = tid % CH;                  // THREADS is a multiple of CH: the same piece of every row
+        auto fetch = [&](int s) __attribute__((always_inline)) {
+            const long k = (long)s * KE + pc * E;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                const int f = i * THREADS + tid, row = f / CH, pc = f % CH;
-                const long k = (long)s * KE + pc * E;
+                const int row = (i * THREADS + tid) / CH;
                 const T* at = row < BM ? A + min(m0 + row, M - 1) * lda : B + (long)min(n0 + (row - BM), N - 1) * ldb;
-                held[i] = whole ? load16(at + k) : load_piece(at, k, K);
+                held[i] = K >= E ? load_tail(at, k, K) : load_piece(at, k, K);
             }
         };
-        auto keep = [&](u32x4* buf) __attribute__((always_inline)) {
+        auto keep = [&](int s) __attribute__((always_inline)) {
+            u32x4* buf = smem + (s & 1) * STAGE;
+            const bool whole = (s + 1) * KE <= K || K < E;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
-                const int f = i * THREADS + tid, row = f / CH, pc = f % CH;
-                buf[row * CH + swizzle<CH>(row < BM ? row : row - BM, pc)] = held[i];
+                const int row = (i * THREADS + tid) / CH;
+                buf[row * CH + swizzle<CH>(row < BM ? row : row - BM, pc)] = whole ? held[i] : tail_fixed<T>(held[i], (long)s * KE + pc * E, K);
             }
         };
-        fetch(0, K >= KE);
-        keep(smem);
+        fetch(0);
+        keep(0);
         __syncthreads();
         for (int s = 0; s < stages; ++s) {
-            if (s + 1 < stages) fetch(s + 1, (s + 2) * KE <= K);
+            if (s + 1 < stages) fetch(s + 1);
             multiply(smem + (s & 1) * STAGE, s + 1 < stages ? CH / 2 : last_steps);
-            if (s + 1 < stages) keep(smem + ((s + 1) & 1) * STAGE);      // read last in the multiplication before this one
+            if (s + 1 < stages) keep(s + 1);      // into the buffer that the multiplication before this one read
             __syncthreads();
         }
     }
@@ -403,23 +460,29 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void rows_gemm_kernel(
     constexpr int LPR = TN / E, RPI = 64 / LPR;   // lanes per row, rows per pass
     const int col = n0 + wn * TN + (lane % LPR) * E;
     const int valid = min(E, N - col);
-    const long oc = (long)g * N + col;
+    const int oc = g * N + col, C = (int)gridDim.y * N;
     float bias[E];
-    load_bias<T>(bias, e, oc, valid);
+    load_bias<T>(bias, e, oc, C);
 #pragma unroll
     for (int j = 0; j < SM; ++j) {
+        const long mj = m0 + wm * TM + j * 32 + lane / LPR;
+        u32x4 add[32 / RPI];
+#pragma unroll
+        for (int r = 0; r < 32 / RPI; ++r)
+            if (e.residual && valid > 0 && C >= E) add[r] = OutRow<T>(e, out, ldo, min(mj + r * RPI, M - 1), C).fetch(oc);
         put_strip<SN>(strip, LD, lane, [&](int i, int r) { return acc[i][j][r]; });
 #pragma unroll
-        for (int r = 0; r < 32; r += RPI) {
-            const int row = r + lane / LPR;
-            const long m = m0 + wm * TM + j * 32 + row;
+        for (int r = 0; r < 32 / RPI; ++r) {
+            const long m = mj + r * RPI;
             float f[E];
 #pragma unroll
             for (int q = 0; q < E; q += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(strip + row * LD + (lane % LPR) * E + q);
+                const float4 v = *reinterpret_cast<const float4*>(strip + (r * RPI + lane / LPR) * LD + (lane % LPR) * E + q);
                 f[q] = v.x, f[q + 1] = v.y, f[q + 2] = v.z, f[q + 3] = v.w;
             }
-            if (m < M && valid > 0) finish_piece<T>(f, bias, out + m * ldo + oc, e, m, oc, valid);
+#pragma unroll
+            for (int q = 0; q < E; ++q) f[q] += bias[q];
+            if (m < M && valid > 0) finish_piece<T>(f, add[r], OutRow<T>(e, out, ldo, m, C), oc, valid, e.act, e.slope);
         }
         wave_sync();
     }
@@ -550,38 +613,39 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void cols_gemm_kernel(const T* __r
     } else {
         constexpr int PIECES = STAGE / THREADS;
         u32x4 held[PIECES];
-        const bool cols_whole = n0 + BC <= N && k0 + BC <= K;
+        const bool cols_whole = n0 + BC <= N && k0 + BC <= K, narrow = N < E || K < E;
         auto fetch = [&](int s) __attribute__((always_inline)) {
-            const bool whole = cols_whole && p_from + (long)(s + 1) * KP <= p_to;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
                 const int q = i * THREADS + tid, in = q < HALF ? q : q - HALF;
-                const int row = in / CP, c = (q < HALF ? n0 : k0) + (in % CP) * E;
-                const long p = p_from + (long)s * KP + row;
+                const int c = (q < HALF ? n0 : k0) + (in % CP) * E, C = q < HALF ? N : K;
+                const long p = min(p_from + (long)s * KP + in / CP, p_to - 1);
                 const T* at = q < HALF ? G + p * ldg : X + p * ldx;
-                if (whole) held[i] = load16(at + c);
-                else {
-                    held[i] = u32x4{0, 0, 0, 0};
-                    if (p < p_to) held[i] = load_piece(at, c, q < HALF ? N : K);
-                }
+                held[i] = narrow ? load_piece(at, c, C) : load_tail(at, c, C);
             }
         };
-        auto keep = [&](u32x4* buf) __attribute__((always_inline)) {
+        auto keep = [&](int s) __attribute__((always_inline)) {
+            u32x4* buf = smem + (s & 1) * STAGE;
+            const long left = p_to - p_from - (long)s * KP;
+            const bool whole = (cols_whole || narrow) && left >= KP;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
                 const int q = i * THREADS + tid, in = q < HALF ? q : q - HALF, row = in / CP;
-                buf[q - in + row * CP + col_swizzle<T, BC>(row, in % CP)] = held[i];
+                u32x4 v = held[i];
+                if (!whole) {
+                    if (!narrow) v = tail_fixed<T>(v, (q < HALF ? n0 : k0) + (in % CP) * E, q < HALF ? N : K);
+                    if (row >= left) v = u32x4{0, 0, 0, 0};
+                }
+                buf[q - in + row * CP + col_swizzle<T, BC>(row, in % CP)] = v;
             }
         };
-        if (stages > 0) {
-            fetch(0);
-            keep(smem);
-        }
+        fetch(0);
+        keep(0);
         __syncthreads();
         for (int s = 0; s < stages; ++s) {
             if (s + 1 < stages) fetch(s + 1);
             multiply(smem + (s & 1) * STAGE);
-            if (s + 1 < stages) keep(smem + ((s + 1) & 1) * STAGE);
+            if (s + 1 < stages) keep(s + 1);
             __syncthreads();
         }
     }
@@ -715,17 +779,329 @@ __global__ __launch_bounds__(256) void transpose_weight_kernel(const T* __restri
     }
 }
 
+// ---- many rows, short k: the weight stays in LDS ---------------------------------------------------------------------------------------
+// With k of a few hundred, the products above spend their time on stages and barriers while memory waits.  Here a workgroup (one per CU, 8
+// waves) keeps a panel of the weight in LDS for all its rows, and every wave for itself takes 32 rows at a time: its piece of x goes straight from
+// memory into the matrix unit's operand registers (lane = row, 16 bytes of k), all of k at once, and is used for every 32 columns of the
+// panel.  x is read once per panel, no barrier after the panel is there, and two waves a SIMD cover each other's loads.
+// The panel is `pg` whole groups, or `pn` columns of one group when that is too large for LDS.
+// Panel rows lie an odd number of pieces apart, so that eight consecutive rows fall on all banks.
+// Results stay in registers: the lane halves of a 32 x 32 tile hold alternate groups of four columns; in 16 bits an exchange between the
+// halves makes that eight consecutive columns, so residual, z and output move as 16-byte pieces.
+// KS: k steps (two pieces each), zeros behind K; LOW: the steps that are whole in every K of this size.
+template <typename T, int LOW, int KS, int THREADS>
+__global__ __launch_bounds__(THREADS, THREADS / 256) void panel_gemm_kernel(const T* __restrict__ X, const T* __restrict__ W, T* __restrict__ out, long M,
+                                                                          int N, int K, int groups, long ldx, long ldw, long ldo, long wg, int pg,
+                                                                          int pn, int parts, Epilogue e) {
+    constexpr int E = Num<T>::E, WAVES = THREADS / 64, PITCH = 2 * KS + 1;
+    extern __shared__ u32x4 smem[];
+    const int npg = (N + pn - 1) / pn;                          // panels per group (1 when a panel holds whole groups)
+    const int g0 = (int)blockIdx.y / npg * pg, g1 = min(groups, g0 + pg);
+    const int n0 = (int)blockIdx.y % npg * pn, n1 = min(N, n0 + pn), rows = n1 - n0, rows32 = (rows + 31) / 32 * 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
+    float* biases = reinterpret_cast<float*>(smem + pg * pn * PITCH);
+    {
+        constexpr int AHEAD = 4;                                // loads in flight per thread
+        const int total = (g1 - g0) * rows * KS * 2;
+        for (int i = threadIdx.x; i < total; i += AHEAD * THREADS) {
+            u32x4 v[AHEAD];
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int q = min(i + j * THREADS, total - 1), row = q / (KS * 2);
+                v[j] = load_tail(W + (g0 + row / rows) * wg + (long)(n0 + row % rows) * ldw, q % (KS * 2) * E, K);
+            }
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int q = i + j * THREADS, pc = q % (KS * 2);
+                if (q < total) smem[q / (KS * 2) * PITCH + pc] = tail_fixed<T>(v[j], pc * E, K);
+            }
+        }
+    }
+    for (int i = threadIdx.x; i < (g1 - g0) * rows32; i += THREADS) {
+        const int n = i % rows32;
+        const long c = (long)(g0 + i / rows32) * N + n0 + n;
+        float b = 0.f;
+        if (e.bias && n < rows) b = e.bias_f32 ? static_cast<const float*>(e.bias)[c] : (float)static_cast<const T*>(e.bias)[c];
+        biases[i] = b;
+    }
+    __syncthreads();
+    const long tiles = (M + 31) / 32;
+    const int C = groups * N;
+    // items: (32 rows, group, part of the panel's columns), rows slowest
+    const int per_row = (g1 - g0) * parts;
+    auto fetch = [&](long item, u32x4 (&x)[KS]) __attribute__((always_inline)) {
+        const T* at = X + min(item / per_row * 32 + r32, M - 1) * ldx + (long)(g0 + (int)(item % per_row) / parts) * K;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x[ks] = ks < LOW ? load16(at + half * E + ks * 2 * E) : load_tail(at, (ks * 2 + half) * E, K);
+    };
+    constexpr bool EARLY = KS <= 17;                            // registers for the next item's x beside this one's
+    const long items = tiles * per_row, stride = (long)gridDim.x * WAVES, first = (long)blockIdx.x * WAVES + wave;
+    u32x4 x[EARLY ? 2 : 1][KS];
+    if (EARLY && first < items) fetch(first, x[0]);
+    auto one = [&](long item, u32x4 (&xi)[KS], u32x4 (&xn)[KS]) __attribute__((always_inline)) {
+        if (EARLY) fetch(min(item + stride, items - 1), xn);
+        else fetch(item, xi);
+        if (K != 2 * KS * E) {                                  // KS is the next size above: zeros behind K
+#pragma unroll
+            for (int ks = LOW; ks < KS; ++ks) xi[ks] = tail_fixed<T>(xi[ks], (ks * 2 + half) * E, K);
+        }
+        const long m = item / per_row * 32 + r32;
+        const OutRow<T> orow(e, out, ldo, min(m, M - 1), C);
+        const int g = g0 + (int)(item % per_row) / parts, part = (int)(item % parts);
+        const int cols = (rows32 / 32 + parts - 1) / parts * 32, c_from = part * cols, c_to = min(rows, c_from + cols);
+        const u32x4* panel = smem + (g - g0) * rows * PITCH + half;
+        const float* bs = biases + (g - g0) * rows32;
+        for (int c0 = c_from; c0 < c_to; c0 += 32) {
+            const u32x4* wrow = panel + min(c0 + r32, rows - 1) * PITCH;
+            u32x4 w[4];                                         // the panel's pieces are read three k steps ahead of the matrix unit
+#pragma unroll
+            for (int ks = 0; ks < 3; ++ks) w[ks] = wrow[min(ks, KS - 1) * 2];
+            f32x16 acc;                                         // bias first: the sums start from it
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 v = *reinterpret_cast<const float4*>(bs + c0 + q * 8 + half * 4);
+                acc[q * 4] = v.x, acc[q * 4 + 1] = v.y, acc[q * 4 + 2] = v.z, acc[q * 4 + 3] = v.w;
+            }
+            const int col0 = g * N + n0 + c0 + half * E;
+            u32x4 add[16 / E];
+            if (e.residual) {
+#pragma unroll
+                for (int q = 0; q < 16 / E; ++q) add[q] = orow.fetch(min(col0 + q * 2 * E, C - 1));
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + 3 < KS) w[(ks + 3) % 4] = wrow[(ks + 3) * 2];
+                __builtin_amdgcn_sched_barrier(0);
+                acc = Num<T>::mma(w[ks % 4], xi[ks], acc);
+            }
+#pragma unroll
+            for (int q = 0; q < 16 / E; ++q) {                  // 16 bits: columns 16 q + 8 half + 0..7; float32: 8 q + 4 half + 0..3
+                float f[E];
+                if constexpr (E == 8) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float lower = acc[q * 8 + j], upper = acc[q * 8 + 4 + j];
+                        const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lower), __builtin_bit_cast(unsigned, upper),
+                                                                           false, false);
+                        const unsigned lo = both[0], hi = both[1];
+                        f[j] = __builtin_bit_cast(float, lo);
+                        f[4 + j] = __builtin_bit_cast(float, hi);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) f[j] = acc[q * 4 + j];
+                }
+                const int valid = min(E, rows - c0 - half * E - q * 2 * E);
+                if (m < M && valid > 0) finish_piece<T>(f, add[q], orow, col0 + q * 2 * E, valid, e.act, e.slope);
+            }
+        }
+    };
+    if constexpr (EARLY) {
+        for (long item = first; item < items; item += 2 * stride) {
+            one(item, x[0], x[1]);
+            if (item + stride < items) one(item + stride, x[1], x[0]);
+        }
+    } else {
+        for (long item = first; item < items; item += stride) one(item, x[0], x[0]);
+    }
+}
+
+constexpr int kPanelLds = 160 * 1024;
+constexpr int panel_threads(int ks) { return ks <= 3 ? 1024 : 512; }      // 128 or 256 registers
+
+// A panel for these sizes; 0 columns: the rows do not fit the registers
+struct PanelPlan {
+    int ks, pg, pn, pitch, panels;
+    size_t lds;
+};
+PanelPlan plan_panel(int N, int K, int groups, size_t S) {
+    PanelPlan p{};
+    const int E = (int)(16 / S), steps = cdiv(K, 2 * E);
+    static const int sizes[] = {3, 6, 9, 13, 17, 25, 34};
+    for (int ks : sizes)
+        if (!p.ks && steps <= ks) p.ks = ks;
+    if (K < E || groups * N < E) p.ks = 0;
+    if (!p.ks) return p;
+    p.pitch = 2 * p.ks + 1;
+    const int room = (kPanelLds - 128) / (p.pitch * 16 + 4);    // columns, each with its bias (those in whole 32s)
+    if (N <= room) {
+        p.pn = N;
+        p.pg = kPanelLds / (N * p.pitch * 16 + cdiv(N, 32) * 128);
+        if (p.pg < 1) p.pg = 1;
+        if (p.pg > groups) p.pg = groups;
+        p.pg = cdiv(groups, cdiv(groups, p.pg));
+        p.panels = cdiv(groups, p.pg);
+    } else {
+        p.pg = 1;
+        const int per = cdiv(N, room / 32 * 32);
+        p.pn = cdiv(cdiv(N, per), 32) * 32;
+        p.panels = groups * cdiv(N, p.pn);
+    }
+    p.lds = (size_t)p.pg * (p.pn * p.pitch * 16 + cdiv(p.pn, 32) * 128);
+    return p;
+}
+
+template <typename T, int LOW, int KS>
+void launch_panel(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
+                  const PanelPlan& p, hipStream_t s) {
+    constexpr int THREADS = panel_threads(KS);
+    auto* kernel = &panel_gemm_kernel<T, LOW, KS, THREADS>;
+    if (p.lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
+    const int per_cu = p.lds <= kPanelLds / 2 && THREADS <= 512 ? 2 : 1;
+    int64_t wgs = cdiv(256 * per_cu, p.panels);
+    if (wgs > cdiv64(M, THREADS / 2)) wgs = cdiv64(M, THREADS / 2);
+    // 32 rows are a large item for a wave that gets one or two of them: the columns in up to four parts, where that evens the waves out
+    const int64_t items = cdiv64(M, 32) * p.pg, waves = wgs * (THREADS / 64);
+    int parts = 1;
+    for (int q = 2; q <= 4 && q * 3 <= cdiv(p.pn, 32); ++q)
+        if (cdiv64(items * q, waves) * parts < cdiv64(items * parts, waves) * q) parts = q;
+    hipLaunchKernelGGL((panel_gemm_kernel<T, LOW, KS, THREADS>), dim3((unsigned)wgs, (unsigned)p.panels), dim3(THREADS), p.lds, s, A, B, out, M, N,
+                       K, groups, lda, ldb, ldo, bg, p.pg, p.pn, parts, e);
+}
+
+template <typename T>
+void panel_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
+                const PanelPlan& p, hipStream_t s) {
+    switch (p.ks) {
+        case 3: return launch_panel<T, 0, 3>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+        case 6: return launch_panel<T, 3, 6>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+        case 9: return launch_panel<T, 6, 9>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+        case 13: return launch_panel<T, 9, 13>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+        case 17: return launch_panel<T, 13, 17>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+        case 25: return launch_panel<T, 17, 25>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+        default: return launch_panel<T, 25, 34>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+    }
+}
+
+// ---- few rows: k split over the waves ----------------------------------------------------------------------------------------------
+// A single row, or a few hundred: too few tiles of the kernels above for 256 CUs, and what counts is how soon the weight arrives.  A workgroup
+// takes 32 rows x 32 columns; its 8 waves take every eighth batch of four k steps (128 bytes of a row), two batches in flight, each for
+// itself: whole 128-byte runs, eight lanes to a row, turned into the operands' order (one row per lane) through LDS of the wave's own.  (Fetched
+// in the operands' order every lane is a request of its own: 11.6 against 7.9 us for 336 x 1296 -> 324 in bfloat16.)  The partial tiles are added through
+// LDS in wave order, then the epilogue runs over whole row pieces, whose bias and residual were fetched before anything else: a
+// dependent trip to memory costs as much as the whole product.  One launch, no workspace.
+template <typename T>
+__global__ __launch_bounds__(512) void few_rows_kernel(const T* __restrict__ X, const T* __restrict__ W, T* __restrict__ out, long M, int N, int K,
+                                                       long ldx, long ldw, long ldo, long wg, Epilogue e) {
+    constexpr int E = Num<T>::E, LD = 36, U = 4, WAVES = 8, LPR = 32 / E;
+    __shared__ u32x4 turn[WAVES][2][32 * 8];              // 64 KB; afterwards the partial tiles
+    const int g = blockIdx.z, n0 = blockIdx.x * 32, C = (int)gridDim.z * N;
+    const long m0 = (long)blockIdx.y * 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5, r8 = lane >> 3, p8 = lane & 7;
+    const T *wrow[U], *xrow[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        wrow[u] = W + g * wg + (long)min(n0 + u * 8 + r8, N - 1) * ldw;
+        xrow[u] = X + min(m0 + u * 8 + r8, M - 1) * ldx + (long)g * K;
+    }
+    const int batches = (K + 2 * U * E - 1) / (2 * U * E), rounds = (batches + WAVES - 1) / WAVES;
+    u32x4 w[3][U], x[3][U];
+    auto fetch = [&](int round, u32x4 (&wb)[U], u32x4 (&xb)[U]) __attribute__((always_inline)) {       // behind K: the row's end
+        const int k = min(((round * WAVES + wave) * 8 + p8) * E, K - E);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            wb[u] = load16(wrow[u] + k);
+            xb[u] = load16(xrow[u] + k);
+        }
+    };
+    fetch(0, w[0], x[0]);
+    // this thread's piece of the result
+    const int prow = threadIdx.x / LPR % 32, pc = threadIdx.x % LPR * E, col = min(g * N + n0 + pc, C - 1), valid = min(E, N - n0 - pc);
+    const bool mine = threadIdx.x < 32 * LPR && m0 + prow < M && valid > 0;
+    const OutRow<T> orow(e, out, ldo, min(m0 + prow, M - 1), C);
+    u32x4 add;
+    float bias[E];
+    if (e.residual && C >= E) add = orow.fetch(col);
+    load_bias<T>(bias, e, col, C);
+    fetch(1, w[1], x[1]);
+    f32x16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+    auto multiply = [&](int round, u32x4 (&wb)[U], u32x4 (&xb)[U]) __attribute__((always_inline)) {
+        const int k0 = (round * WAVES + wave) * U * 2 * E;
+        if (k0 + U * 2 * E > K) {              // zeros behind K
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                wb[u] = tail_fixed<T>(wb[u], k0 + p8 * E, K);
+                xb[u] = tail_fixed<T>(xb[u], k0 + p8 * E, K);
+            }
+        }
+        u32x4 *wt = turn[wave][0], *xt = turn[wave][1];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            wt[(u * 8 + r8) * 8 + swizzle<8>(r8, p8)] = wb[u];
+            xt[(u * 8 + r8) * 8 + swizzle<8>(r8, p8)] = xb[u];
+        }
+        wave_sync();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            acc = Num<T>::mma(wt[r32 * 8 + swizzle<8>(r32, u * 2 + half)], xt[r32 * 8 + swizzle<8>(r32, u * 2 + half)], acc);
+        wave_sync();
+    };
+    for (int r = 0;;) {
+        fetch(r + 2, w[2], x[2]);
+        multiply(r, w[0], x[0]);
+        if (++r == rounds) break;
+        fetch(r + 2, w[0], x[0]);
+        multiply(r, w[1], x[1]);
+        if (++r == rounds) break;
+        fetch(r + 2, w[1], x[1]);
+        multiply(r, w[2], x[2]);
+        if (++r == rounds) break;
+    }
+    __syncthreads();
+    float(*part)[32][LD] = reinterpret_cast<float(*)[32][LD]>(&turn[0][0][0]);
+    static_assert(sizeof(float) * WAVES * 32 * LD <= sizeof(turn), "the partial tiles lie in the waves' LDS");
+    put_strip<1>(&part[wave][0][0], LD, lane, [&](int, int r) { return acc[r]; });
+    __syncthreads();
+    if (!mine) return;
+    float f[E];
+#pragma unroll
+    for (int q = 0; q < E; q += 4) {
+        float4 t = *reinterpret_cast<const float4*>(&part[0][prow][pc + q]);
+#pragma unroll
+        for (int v = 1; v < WAVES; ++v) {
+            const float4 o = *reinterpret_cast<const float4*>(&part[v][prow][pc + q]);
+            t.x += o.x, t.y += o.y, t.z += o.z, t.w += o.w;
+        }
+        f[q] = t.x + bias[q], f[q + 1] = t.y + bias[q + 1], f[q + 2] = t.z + bias[q + 2], f[q + 3] = t.w + bias[q + 3];
+    }
+    finish_piece<T>(f, add, orow, g * N + n0 + pc, valid, e.act, e.slope);
+}
+
+template <typename T>
+void launch_few_rows(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
+                     hipStream_t s) {
+    const dim3 grid((unsigned)cdiv(N, 32), (unsigned)cdiv64(M, 32), (unsigned)groups);
+    hipLaunchKernelGGL(few_rows_kernel<T>, grid, dim3(512), 0, s, A, B, out, M, N, K, lda, ldb, ldo, bg, e);
+}
+
 // ---- plans ---------------------------------------------------------------------------------------------------------------------------
 size_t elem_bytes(int dtype) { return dtype == 0 ? 4 : 2; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+constexpr long kPanelRows = 16384;
+
+constexpr long kBigTiles = 128;          // 256 x 256 tiles from which they are worth half the CUs standing idle
+constexpr long kFewTiles = 128;
 
 template <typename T>
 void rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
                hipStream_t s) {
     constexpr size_t S = sizeof(T);
     const bool dma = on16(A, lda, S) && on16(B, ldb, S) && (long)K * S % 16 == 0 && bg * (long)S % 16 == 0;
+    const PanelPlan p = plan_panel(N, K, groups, S);
+    if (p.ks && M >= kPanelRows) {
+        panel_gemm<T>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+        return;
+    }
+    if (K >= Num<T>::E && (M <= 32 || cdiv64(M, 64) * cdiv(N, 64) * groups < kFewTiles)) {
+        launch_few_rows<T>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+        return;
+    }
     const int64_t big = cdiv64(M, 128) * cdiv(N, 128) * groups;
-    if (dma && big >= 256) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    if (dma && cdiv64(M, 256) * cdiv(N, 256) * groups >= kBigTiles) launch_rows_gemm<T, 256, 256, 2, 4, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else if (dma && big >= 256) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
     else if (dma) launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
     else if (big >= 256) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
     else launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
@@ -864,24 +1240,14 @@ int check_sizes(const char* who, int64_t P, int N, int K, int groups, int dtype,
 
 using namespace nextou;
 
-extern "C" int nextou_linear_act_fwd_workspace(int64_t P, int N, int K, int groups, int dtype, size_t* bytes) {
-    if (int e = check_sizes("linear_act_fwd_workspace", P, N, K, groups, dtype, 0)) return e;
-    NEXTOU_REQUIRE(bytes, "linear_act_fwd_workspace: null pointer");
-    *bytes = 0;
-    return 0;
-}
-
 extern "C" int nextou_linear_act_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre,
-                                     void* workspace, size_t workspace_bytes, int64_t P, int N, int K, int groups, int64_t ldx, int64_t ldr,
+                                     int64_t P, int N, int K, int groups, int64_t ldx, int64_t ldr,
                                      int64_t ldy, int dtype, int bias_f32, int act, float slope, nextou_stream_t stream) {
     if (int e = check_sizes("linear_act_fwd", P, N, K, groups, dtype, act)) return e;
     NEXTOU_REQUIRE(x && w && y, "linear_act_fwd: null pointer");
     NEXTOU_REQUIRE(ldx >= 0 && ldr >= 0 && ldy >= (int64_t)groups * N, "linear_act_fwd: bad row strides %lld, %lld, %lld", (long long)ldx,
                    (long long)ldr, (long long)ldy);
-    size_t need = 0;
-    nextou_linear_act_fwd_workspace(P, N, K, groups, dtype, &need);
-    if (workspace_bytes < need) return fail(NEXTOU_ENOSPACE, "linear_act_fwd: workspace %zu < %zu bytes", workspace_bytes, need);
-    const Epilogue e{bias, bias_f32, residual, (long)ldr, pre, (long)groups * N, act, slope};
+    const Epilogue e{bias, bias_f32, residual, (long)ldr, pre, act, slope};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case 0: return launch_fwd<float>((const float*)x, (const float*)w, (float*)y, P, N, K, groups, ldx, ldy, e, s);

@@ -75,6 +75,14 @@ def _f32c(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+_NO_CONTEXT = contextlib.nullcontext()
+
+
+def _current_device(device: torch.device):
+    """``torch.cuda.device(device)``, without its cost where that is the current one."""
+    return _NO_CONTEXT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -895,20 +903,17 @@ class _HipBackend:
     @staticmethod
     def linear_act_fwd(x, w, bias, residual, act, slope, groups, want_pre):
         """x (P, groups*K) rows with dense columns, w (groups*N, K) dense -> (y (P, groups*N) dense, z for the backward | None)."""
-        import ctypes
-        L_ = _lib.lib()
-        P, (C, K) = x.shape[0], w.shape
-        N, code = C // groups, _LINEAR_TYPES[x.dtype]
-        need = ctypes.c_size_t(0)
-        with torch.cuda.device(x.device):
-            _lib.check(L_.nextou_linear_act_fwd_workspace(P, N, K, groups, code, ctypes.byref(need)), "linear_act_fwd_workspace")
-            ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
-            y = torch.empty((P, C), dtype=x.dtype, device=x.device)
-            pre = torch.empty((P, C), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device) if want_pre else None
-            rc = L_.nextou_linear_act_fwd(x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(pre), _ptr(ws), need.value,
-                                          P, N, K, groups, x.stride(0), 0 if residual is None else residual.stride(0), C, code,
-                                          int(bias is not None and bias.dtype == torch.float32), act, slope, _stream_ptr(x.device))
-        _lib.check(rc, "linear_act_fwd")
+        P, (C, K), dev = x.shape[0], w.shape, x.device
+        with _current_device(dev):
+            y = torch.empty((P, C), dtype=x.dtype, device=dev)
+            pre = torch.empty((P, C), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=dev) if want_pre else None
+            rc = _lib.lib().nextou_linear_act_fwd(
+                x.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
+                y.data_ptr(), None if pre is None else pre.data_ptr(), P, C // groups, K, groups, x.stride(0),
+                0 if residual is None else residual.stride(0), C, _LINEAR_TYPES[x.dtype], bias is not None and bias.dtype == torch.float32,
+                act, slope, _stream_ptr(dev))
+        if rc:
+            _lib.check(rc, "linear_act_fwd")
         return y, pre
 
     @staticmethod
@@ -919,7 +924,7 @@ class _HipBackend:
         P, (C, K) = x.shape[0], w.shape
         N, code = C // groups, _LINEAR_TYPES[x.dtype]
         need = ctypes.c_size_t(0)
-        with torch.cuda.device(x.device):
+        with _current_device(x.device):
             _lib.check(L_.nextou_linear_act_bwd_workspace(P, N, K, groups, code, act, int(want_gx), int(want_gw), int(gb_dtype is not None),
                                                           ctypes.byref(need)), "linear_act_bwd_workspace")
             ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
@@ -1784,7 +1789,7 @@ _LINEAR_ACTS = {"none": 0, "relu": 1, "leakyrelu": 2, "gelu": 3, "hswish": 4, "h
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
     """(..., C) -> (P, C) with dense columns and one row stride: a view where the strides allow one (an expanded row included), else a copy."""
-    rows = t.reshape(-1, t.shape[-1])
+    rows = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     return rows if rows.shape[1] == 1 or rows.stride(1) == 1 else rows.contiguous()
 
 
@@ -1793,7 +1798,7 @@ class _LinearAct(torch.autograd.Function):
     LeakyReLU without a shortcut; float16 apart, whose small positive values can round to zero); else z, written by the same launch."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, slope, groups, training):
+    def forward(ctx, x, weight, bias, residual, act, slope, groups):
         be = _backend_for(x)
         if x.numel() == 0:
             ctx.save_for_backward(x, weight, None)
@@ -1801,12 +1806,11 @@ class _LinearAct(torch.autograd.Function):
             return x.new_empty(x.shape[:-1] + (weight.shape[0],))
         x2, w2 = _as_rows(x), weight.contiguous()
         sign = act == 1 or (act == 2 and slope >= 0.0)
-        kind = 0 if act == 0 or not training else (2 if sign and residual is None and x.dtype != torch.float16 else 1)
+        kind = 0 if act == 0 else (2 if sign and residual is None and x.dtype != torch.float16 else 1)
         y, pre = be.linear_act_fwd(x2, w2, bias, None if residual is None else _as_rows(residual), act, slope, groups, kind == 1)
         y = y.view(x.shape[:-1] + (w2.shape[0],))
-        if training:
-            ctx.save_for_backward(x, weight, pre if kind == 1 else (y if kind == 2 else None))
-            ctx.conf = (kind, act, slope, groups, None if bias is None else bias.dtype)
+        ctx.save_for_backward(x, weight, pre if kind == 1 else (y if kind == 2 else None))
+        ctx.conf = (kind, act, slope, groups, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
@@ -1824,7 +1828,7 @@ class _LinearAct(torch.autograd.Function):
                 _as_rows(gy), _as_rows(x), weight.contiguous(), None if saved is None else saved.reshape(-1, weight.shape[0]), kind, act,
                 slope, groups, want_x, want_w, bias_dtype if want_b else None)
         return (None if gx is None else gx.view(x.shape), None if gw is None else gw.view(weight.shape), gb,
-                gy if ctx.needs_input_grad[3] else None, None, None, None, None)
+                gy if ctx.needs_input_grad[3] else None, None, None, None)
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -1862,9 +1866,13 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
             (bias is not None and bias.dtype not in (x.dtype, torch.float32)):
         raise TypeError("linear_act: float32, bfloat16 or float16 tensors of one type (a float32 bias apart), got %s" %
                         ", ".join(str(t.dtype) for t in given))
+    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     training = torch.is_grad_enabled() and any(t.requires_grad for t in given)
-    return _LinearAct.apply(x, weight, None if bias is None else bias.contiguous(), residual, _LINEAR_ACTS[act], float(negative_slope), groups,
-                            training)
+    if not training and x.numel():
+        y, _ = _backend_for(x).linear_act_fwd(_as_rows(x), weight.contiguous(), bias, None if residual is None else _as_rows(residual),
+                                              _LINEAR_ACTS[act], float(negative_slope), groups, False)
+        return y if x.dim() == 2 else y.view(x.shape[:-1] + (weight.shape[0],))
+    return _LinearAct.apply(x, weight, bias, residual, _LINEAR_ACTS[act], float(negative_slope), groups)
 
 
 def pointwise_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,

@@ -105,9 +105,9 @@ def test_there_is_no_cpu_implementation():
 
 def test_c_entries_check_their_arguments():
     L, n = _lib.lib(), ctypes.c_size_t(0)
-    fwd = lambda **k: L.nextou_linear_act_fwd(*[{**dict(x=16, w=16, b=None, r=None, y=16, pre=None, ws=None, wsb=0, P=1, N=1, K=1, g=1, ldx=1,  # noqa: E731
+    fwd = lambda **k: L.nextou_linear_act_fwd(*[{**dict(x=16, w=16, b=None, r=None, y=16, pre=None, P=1, N=1, K=1, g=1, ldx=1,  # noqa: E731
                                                         ldr=0, ldy=1, dt=0, bf=0, act=0, s=0.0, st=None), **k}[i] for i in
-                                                "x w b r y pre ws wsb P N K g ldx ldr ldy dt bf act s st".split()])
+                                                "x w b r y pre P N K g ldx ldr ldy dt bf act s st".split()])
     assert fwd(x=None) == -1 and b"null" in L.nextou_last_error()
     assert fwd(P=0) == -1 and fwd(N=0) == -1 and fwd(K=-1) == -1 and fwd(g=0) == -1 and fwd(dt=3) == -1 and fwd(act=5) == -1
     assert fwd(N=4, ldy=3) == -1 and b"stride" in L.nextou_last_error()
@@ -119,7 +119,6 @@ def test_c_entries_check_their_arguments():
     assert bwd(act=3, kind=2, sv=16) == -1 and b"sign" in L.nextou_last_error()
     assert bwd(act=2, kind=2, sv=16, s=-0.5) == -1
     assert bwd(act=3, kind=1, sv=16) == -2 and b"workspace" in L.nextou_last_error()
-    assert L.nextou_linear_act_fwd_workspace(4, 4, 4, 1, 1, None) == -1
     assert L.nextou_linear_act_bwd_workspace(4, 4, 4, 1, 9, 0, 1, 1, 1, ctypes.byref(n)) == -1
 
     assert L.nextou_multi_norm_workspace(0, ctypes.byref(n)) == -1
