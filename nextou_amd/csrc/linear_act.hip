@@ -20,23 +20,22 @@ enum Act { kActNone = 0, kActRelu = 1, kActLeaky = 2, kActGelu = 3, kActHardswis
 // ---- activations --------------------------------------------------------------------------------------------------------------------
 constexpr float kInvSqrt2 = 0.70710678118654752f, kInvSqrt2Pi = 0.39894228040143268f;
 
-// Phi(z), and e = exp(-z^2 / 2) beside it.  float32 rows: the library's erfc (relative accuracy in both tails).  16-bit rows: Abramowitz and
-// Stegun 7.1.26 (|error| <= 1.5e-7 of erf), five multiply-adds, one exp and one reciprocal instead of some forty instructions.
+// The normal distribution's tail Phi(-|z|), and e = exp(-z^2 / 2) beside it.  float32 rows: the library's erfc (relative accuracy all the
+// way).  16-bit rows: Abramowitz and Stegun 7.1.26 (|error| <= 1.5e-7 of erf): five multiply-adds, one exp and one reciprocal, since the epilogue
+// of a product that the matrix units finish in microseconds is bound by exactly these instructions.
 template <bool FAST>
-__device__ __forceinline__ float normal_cdf(float z, float* e) {
+__device__ __forceinline__ float normal_tail(float z, float* e) {
     if constexpr (FAST) {
-        const float a = fabsf(z) * kInvSqrt2;
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.f));
-        float q = fmaf(1.061405429f, t, -1.453152027f);
-        q = fmaf(q, t, 1.421413741f);
-        q = fmaf(q, t, -0.284496736f);
-        q = fmaf(q, t, 0.254829592f);
-        *e = __expf(-a * a);
-        const float tail = 0.5f * q * t * *e;
-        return z < 0.f ? tail : 1.f - tail;
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * kInvSqrt2, fabsf(z), 1.f));
+        float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+        q = fmaf(q, t, 0.5f * 1.421413741f);
+        q = fmaf(q, t, 0.5f * -0.284496736f);
+        q = fmaf(q, t, 0.5f * 0.254829592f);
+        *e = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.44269504f));
+        return q * t * *e;
     } else {
         *e = expf(-0.5f * z * z);
-        return 0.5f * erfcf(-z * kInvSqrt2);
+        return 0.5f * erfcf(fabsf(z) * kInvSqrt2);
     }
 }
 
@@ -57,8 +56,10 @@ __device__ __forceinline__ void activate(float (&f)[E], int act, float slope) {
     } else if (act == kActGelu) {
 #pragma unroll
         for (int i = 0; i < E; ++i) {
+            // z Phi(z) = max(z, 0) - |z| Phi(-|z|); the tail is 0 long before 1e4 (and stays so at infinity)
             float e;
-            f[i] *= normal_cdf<FAST>(f[i], &e);
+            const float z = f[i], tail = normal_tail<FAST>(z, &e);
+            f[i] = fmaf(-fminf(fabsf(z), 1e4f), tail, z < 0.f ? 0.f : z);
         }
     } else if (act == kActHardswish) {
 #pragma unroll
@@ -74,8 +75,8 @@ __device__ __forceinline__ float act_slope(float z, int act, float slope) {
         case kActGelu: {
             const float c = z > 40.f ? 40.f : (z < -40.f ? -40.f : z);      // beyond that z phi(z) is 0 and must not become inf * 0
             float e;
-            const float cdf = normal_cdf<FAST>(c, &e);
-            return fmaf(c * kInvSqrt2Pi, e, cdf);
+            const float tail = normal_tail<FAST>(c, &e);
+            return fmaf(c * kInvSqrt2Pi, e, c < 0.f ? tail : 1.f - tail);
         }
         case kActHardswish: return z <= -3.f ? 0.f : (z >= 3.f ? 1.f : fmaf(2.f, z, 3.f) * (1.f / 6.f));
         default: return 1.f;
@@ -680,25 +681,34 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void cols_gemm_kernel(const T* __r
 }
 
 // out[i] = sum over splits of partial[split][i], in a fixed order: `parts` threads take a contiguous run of the splits each (one when there
-// are few: then every thread reads whole lines), and their sums are added in order
+// are few: then every thread reads whole lines), and their sums are added in order.  Two such sums in one launch: the bias's and the weight's.
+struct SplitSum {
+    const float* partial;
+    void* out;
+    int out_f32, splits, parts;
+    long n;
+    unsigned blocks;
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void split_sum_kernel(const float* __restrict__ partial, void* __restrict__ out, int out_f32, long n, int splits,
-                                                        int parts) {
+__global__ __launch_bounds__(256) void split_sum_kernel(SplitSum first, SplitSum second) {
     __shared__ float sums[256];
-    const int per = 256 / parts, part = threadIdx.x / per;
-    const long i = (long)blockIdx.x * per + threadIdx.x % per;
-    const int from = (int)((long)splits * part / parts), to = (int)((long)splits * (part + 1) / parts);
+    const bool is_first = blockIdx.x < first.blocks;
+    const SplitSum& a = is_first ? first : second;
+    const int per = 256 / a.parts, part = threadIdx.x / per;
+    const long i = (long)(is_first ? blockIdx.x : blockIdx.x - first.blocks) * per + threadIdx.x % per;
+    const int from = (int)((long)a.splits * part / a.parts), to = (int)((long)a.splits * (part + 1) / a.parts);
     float t = 0.f;
-    if (i < n) {
+    if (i < a.n) {
 #pragma unroll 8
-        for (int s = from; s < to; ++s) t += partial[s * n + i];
+        for (int s = from; s < to; ++s) t += a.partial[s * a.n + i];
     }
     sums[threadIdx.x] = t;
     __syncthreads();
-    if (part != 0 || i >= n) return;
-    for (int q = 1; q < parts; ++q) t += sums[q * per + threadIdx.x];
-    if (out_f32) static_cast<float*>(out)[i] = t;
-    else static_cast<T*>(out)[i] = (T)t;
+    if (part != 0 || i >= a.n) return;
+    for (int q = 1; q < a.parts; ++q) t += sums[q * per + threadIdx.x];
+    if (a.out_f32) static_cast<float*>(a.out)[i] = t;
+    else static_cast<T*>(a.out)[i] = (T)t;
 }
 
 // ---- the activation's gradient and the column sums ------------------------------------------------------------------------------------
@@ -768,14 +778,28 @@ __global__ __launch_bounds__(256) void transpose_weight_kernel(const T* __restri
     const int n0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
     w += (long)blockIdx.z * N * K;
     wt += (long)blockIdx.z * K * ldt;
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const int n = n0 + i / 64, k = k0 + i % 64;
-        tile[i / 64][i % 64] = n < N && k < K ? w[(long)n * K + k] : (T)0.f;
+    constexpr int E = Num<T>::E, LPR = 64 / E;
+#pragma unroll
+    for (int j = 0; j < 64 * LPR / 256; ++j) {
+        const int i = j * 256 + threadIdx.x, r = i / LPR, c = i % LPR * E;
+        T v[E];
+        u32x4 piece{0, 0, 0, 0};
+        if (n0 + r < N && k0 + c < K) piece = load_piece(w + (long)(n0 + r) * K, k0 + c, K);
+        __builtin_memcpy(v, &piece, 16);
+#pragma unroll
+        for (int q = 0; q < E; ++q) tile[r][c + q] = v[q];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const int k = k0 + i / 64, n = n0 + i % 64;
-        if (k < K && n < ldt) wt[(long)k * ldt + n] = tile[i % 64][i / 64];
+#pragma unroll
+    for (int j = 0; j < 64 * LPR / 256; ++j) {
+        const int i = j * 256 + threadIdx.x, r = i / LPR, c = i % LPR * E;
+        if (k0 + r >= K || n0 + c >= ldt) continue;             // ldt is a whole number of pieces
+        T v[E];
+        u32x4 piece;
+#pragma unroll
+        for (int q = 0; q < E; ++q) v[q] = tile[c + q][r];
+        __builtin_memcpy(&piece, v, 16);
+        store16(wt + (long)(k0 + r) * ldt + n0 + c, piece);
     }
 }
 
@@ -1082,8 +1106,16 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 constexpr long kPanelRows = 16384;
 
-constexpr long kBigTiles = 128;          // 256 x 256 tiles from which they are worth half the CUs standing idle
 constexpr long kFewTiles = 128;
+
+// Rounds of the CUs that square tiles of three sizes need, in units of a 64 x 64 tile's matrix work; what a CU holds at a time is one 256, two
+// 128 or four 64 tiles.  Weighted by what they reach when they fill the card (16384 x 2048 -> 8192 in bfloat16: 1030, 900, 620 TFLOP/s).
+int tile_size(long M, int N, int groups, bool dma) {
+    const auto rounds = [&](long t, long at_a_time) { return (cdiv64(M, t) * cdiv64(N, t) * groups + 256 * at_a_time - 1) / (256 * at_a_time); };
+    const double c256 = 16.0 * rounds(256, 1) / 1.03, c128 = 8.0 * rounds(128, 2) / 0.9, c64 = 4.0 * rounds(64, 4) / 0.62;
+    if (dma && c256 <= c128 && c256 <= c64) return 256;
+    return c128 <= c64 ? 128 : 64;
+}
 
 template <typename T>
 void rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
@@ -1099,11 +1131,11 @@ void rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups,
         launch_few_rows<T>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
         return;
     }
-    const int64_t big = cdiv64(M, 128) * cdiv(N, 128) * groups;
-    if (dma && cdiv64(M, 256) * cdiv(N, 256) * groups >= kBigTiles) launch_rows_gemm<T, 256, 256, 2, 4, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else if (dma && big >= 256) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    const int tile = tile_size(M, N, groups, dma);
+    if (tile == 256) launch_rows_gemm<T, 256, 256, 2, 4, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else if (dma && tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
     else if (dma) launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else if (big >= 256) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else if (tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
     else launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
 }
 
@@ -1137,10 +1169,9 @@ void launch_cols_gemm(const T* G, const T* X, T* out, float* partial, long P, in
                        ldx, p.nt, p.kt, p.rows_per_split);
 }
 
-template <typename T>
-void split_sum(const float* partial, void* out, int out_f32, long n, int splits, hipStream_t s) {
+SplitSum split_sum(const float* partial, void* out, int out_f32, long n, int splits) {
     const int parts = splits >= 64 ? 16 : (splits >= 16 && n < 65536 ? 4 : 1);
-    hipLaunchKernelGGL(split_sum_kernel<T>, dim3((unsigned)cdiv64(n, 256 / parts)), dim3(256), 0, s, partial, out, out_f32, n, splits, parts);
+    return SplitSum{partial, out, out_f32, splits, parts, n, (unsigned)cdiv64(n, 256 / parts)};
 }
 
 // `padded`: G's rows are followed by zeros up to whole pieces
@@ -1154,7 +1185,6 @@ void cols_gemm(const T* G, const T* X, T* out, float* partial, long P, int N, in
     else if (p.bc == 128) launch_cols_gemm<T, 128, 0>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
     else if (dma) launch_cols_gemm<T, 64, 1>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
     else launch_cols_gemm<T, 64, 0>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
-    if (p.splits > 1) split_sum<T>(partial, out, 0, (long)groups * N * K, p.splits, s);
 }
 
 // Workspace of a backward call: [dz][transposed weight][column sums][split blocks]
@@ -1172,9 +1202,13 @@ BwdPlan plan_bwd(int64_t P, int N, int K, int groups, int dtype, int act, bool w
     const int64_t C = (int64_t)groups * N;
     b.ld_dz = cdiv64(C, E) * E;
     b.ldt = cdiv(N, E) * E;
+    // lanes per row: the division of the row's pieces (at least 16 together, 256 bytes) that leaves the fewest of 256 threads idle
     const int64_t pieces = b.ld_dz / E;
-    b.col_blocks = (int)cdiv64(pieces, 256);
-    b.lanes = (int)cdiv64(pieces, b.col_blocks);
+    int64_t best = 0;
+    for (int64_t cb = cdiv64(pieces, 256); cb == 1 || (cb <= cdiv64(pieces, 256) + 16 && cdiv64(pieces, cb) >= 16); ++cb) {
+        const int64_t lanes = cdiv64(pieces, cb), used = 256 / lanes * pieces * 1000 / cb;
+        if (used > best + best / 50) best = used, b.col_blocks = (int)cb, b.lanes = (int)lanes;
+    }
     const int rows = 256 / b.lanes;                       // rows a workgroup holds at a time; at least 8 of them each, about 1024 workgroups
     int64_t blocks = cdiv64(1024, b.col_blocks), most = cdiv64(P, 8 * rows);
     if (blocks > most) blocks = most;
@@ -1209,7 +1243,6 @@ int launch_bwd(const T* gy, const T* x, const T* w, const void* saved, int kind,
         auto* kernel = kind == 0 ? &act_grad_kernel<T, 0> : (kind == 1 ? &act_grad_kernel<T, 1> : &act_grad_kernel<T, 2>);
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, gy, saved, dz, sums, (long)P, (long)C, (long)ldg, (long)b.ld_dz, b.lanes,
                            (long)b.rows_per_block, act, slope);
-        if (sums) split_sum<T>(sums, gb, gb_f32, C, b.row_blocks, s);
     }
     const bool padded = dz != nullptr;
     if (padded) {
@@ -1223,6 +1256,12 @@ int launch_bwd(const T* gy, const T* x, const T* w, const void* saved, int kind,
         rows_gemm<T>(gy, wt, gx, P, K, padded && groups == 1 ? b.ldt : N, groups, ldg, b.ldt, (long)groups * K, (long)K * b.ldt, none, s);
     }
     if (gw) cols_gemm<T>(gy, x, gw, split, P, N, K, groups, ldg, ldx, padded, dtype, s);
+    SplitSum first{}, second{};
+    first.parts = second.parts = 1;
+    if (gb) first = split_sum(sums, gb, gb_f32, C, b.row_blocks);
+    if (b.split) second = split_sum(split, gw, 0, (long)groups * N * K, b.cols.splits);
+    if (first.blocks + second.blocks)
+        hipLaunchKernelGGL(split_sum_kernel<T>, dim3(first.blocks + second.blocks), dim3(256), 0, s, first, second);
     return check_launch("linear_act_bwd");
 }
 
