@@ -190,20 +190,23 @@ template <typename T>
 __device__ __forceinline__ u32x4 load_tail(const T* row, long c, long C) {
     return load16(row + min(c, C - Num<T>::E));
 }
+// (In 32-bit steps: with 64-bit shifts by a register the compiler put the shift count into the last register of the kernel's allocation,
+// and the results were wrong now and then — garbage in about one of thirty runs of the float32 few_rows_kernel, gone with these.)
 template <typename T>
 __device__ __forceinline__ u32x4 tail_fixed(u32x4 v, long c, long C) {
-    constexpr int E = Num<T>::E, BITS = 8 * sizeof(T);
-    const int over = (int)max(0l, min((long)E, c + E - C)) * BITS;      // bits to drop: 0 ... 128
-    unsigned long long lo = v[0] | (unsigned long long)v[1] << 32, hi = v[2] | (unsigned long long)v[3] << 32;
-    if (over >= 64) {
-        lo = hi;
-        hi = 0;
+    constexpr int E = Num<T>::E;
+    int drop = (int)max(0l, min((long)E, c + E - C));                   // elements: 0 ... E
+    unsigned a0 = v[0], a1 = v[1], a2 = v[2], a3 = v[3];
+    if constexpr (E == 8) {
+        const bool odd = drop & 1;
+        const unsigned b0 = a0 >> 16 | a1 << 16, b1 = a1 >> 16 | a2 << 16, b2 = a2 >> 16 | a3 << 16, b3 = a3 >> 16;
+        a0 = odd ? b0 : a0, a1 = odd ? b1 : a1, a2 = odd ? b2 : a2, a3 = odd ? b3 : a3;
+        drop >>= 1;
     }
-    const int sh = over & 63;
-    lo = sh ? lo >> sh | hi << (64 - sh) : lo;
-    hi >>= sh;
-    if (over == 128) lo = 0;
-    return u32x4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
+    const bool one = drop & 1, two = drop & 2, all = drop & 4;
+    a0 = one ? a1 : a0, a1 = one ? a2 : a1, a2 = one ? a3 : a2, a3 = one ? 0 : a3;
+    a0 = two ? a2 : a0, a1 = two ? a3 : a1, a2 = two ? 0 : a2, a3 = two ? 0 : a3;
+    return u32x4{all ? 0 : a0, all ? 0 : a1, all ? 0 : a2, all ? 0 : a3};
 }
 
 // ---- rows times rows: out[m, n] = sum_k A[m, k] B[n, k], both k-contiguous ------------------------------------------------------------
@@ -211,8 +214,8 @@ __device__ __forceinline__ u32x4 tail_fixed(u32x4 v, long c, long C) {
 //
 // A workgroup of WR x WC waves computes BM x BN outputs; a wave its (BM / WR) x (BN / WC) block out of 32 x 32 matrix-unit tiles, n in the
 // tile's rows: a lane ends up with four consecutive n of one m.  k advances in stages of CH 16-byte pieces per row (CH = 8: 64 sixteen-bit
-// or 32 float values), kept in LDS as [row][piece] with the piece index XORed by the row, so that the eight lanes that are served
-// together read eight different 16-byte columns.  In float32 a piece feeds four matrix instructions, in 16 bits one: the same addresses.
+// or 32 float values), kept in LDS as [row][piece] with the piece index XORed by the row, so that the sixteen lanes that are served
+// together (16 rows, one piece) fall on all sixteen 16-byte columns of the 64 banks.  In float32 a piece feeds four matrix instructions, in 16 bits one: the same addresses.
 //
 // DMA = 1: every row starts on 16 bytes and K is a whole number of pieces; stages go from memory to LDS without registers
 // (global_load_lds), NBUF - 1 stages ahead, one barrier a stage.  Rows behind the end are read from the last row (their outputs are not
@@ -235,8 +238,8 @@ struct Epilogue {
 
 template <int CH>
 __device__ __forceinline__ int swizzle(int row, int piece) {
-    if constexpr (CH == 8) return piece ^ (row & 7);
-    else return piece ^ ((row >> 1) & 3);
+    if constexpr (CH == 8) return piece ^ ((row >> 1) & 7);
+    else return piece ^ ((row >> 2) & 3);
 }
 
 // LDS written by a wave is read by the same wave's other lanes behind this (its LDS instructions run in order)
@@ -1053,8 +1056,8 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const T* __restrict__ X, 
         u32x4 *wt = turn[wave][0], *xt = turn[wave][1];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            wt[(u * 8 + r8) * 8 + swizzle<8>(r8, p8)] = wb[u];
-            xt[(u * 8 + r8) * 8 + swizzle<8>(r8, p8)] = xb[u];
+            wt[(u * 8 + r8) * 8 + swizzle<8>(u * 8 + r8, p8)] = wb[u];
+            xt[(u * 8 + r8) * 8 + swizzle<8>(u * 8 + r8, p8)] = xb[u];
         }
         wave_sync();
 #pragma unroll

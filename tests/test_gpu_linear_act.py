@@ -180,6 +180,19 @@ def test_repeats_are_bit_identical(ops, t):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("P,K,N,groups", [(6, 136, 200, 1), (300, 99, 187, 1), (20000, 44, 44, 2), (20000, 132, 72, 1), (700, 331, 130, 1)])
+def test_many_calls_give_one_result(ops, P, K, N, groups, t):
+    """Rows that end inside a 16-byte piece or a stage, two hundred calls in a row (whole numbers: the sums are exact, so is the comparison)."""
+    g = torch.Generator().manual_seed(K)
+    x = torch.randint(-3, 4, (P, groups * K), generator=g).to(t).to(DEV)
+    w = torch.randint(-3, 4, (groups * N, K), generator=g).to(t).to(DEV)
+    want = _mm(x.double(), w.double(), groups).to(t)
+    with torch.no_grad():
+        wrong = sum((ops.linear_act(x, w, groups=groups) != want).any().int() for _ in range(200))
+    assert int(wrong) == 0
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
 @pytest.mark.parametrize("P,K,N", [(37, 50, 35), (150, 128, 72), (260, 264, 136), (3, 515, 129)])
 def test_strides_offsets_and_surroundings(ops, P, K, N, t):
     """Rows inside wider tensors at odd offsets, transposed operands, expanded rows; everything around the operands is NaN, so a value read from
