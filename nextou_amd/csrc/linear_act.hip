@@ -337,7 +337,7 @@ __device__ __forceinline__ void load_bias(float (&b)[Num<T>::E], const Epilogue&
 }
 
 template <typename T, int BM, int BN, int WR, int WC, int CH, int NBUF, int DMA>
-__global__ __launch_bounds__(64 * WR * WC, 2) void rows_gemm_kernel(
+__global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 : 2) void rows_gemm_kernel(
     const T* __restrict__ A, const T* __restrict__ B, T* __restrict__ out, long M, int N, int K, long lda, long ldb, long ldo, long bg, int mt, int nt,
     Epilogue e) {
     constexpr int E = Num<T>::E, KE = CH * E, THREADS = 64 * WR * WC, WAVES = WR * WC;
@@ -410,18 +410,49 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void rows_gemm_kernel(
                                                  (__attribute__((address_space(3))) void*)(buf + (i * WAVES + wave) * 64), 16, 0, 0);
             }
         };
+        // The operands of a k step are read from LDS while the step before it is multiplied, across the stages as well: the barrier that
+        // hands a stage over stands in front of the LAST step's multiplication, whose operands are in registers by then, so the buffer
+        // just read is free for the stage after the next, and the first operands of the next stage arrive behind the multiplication.
+        u32x4 a[2][SM], b[2][SN];
+        auto read = [&](int s, int ks, u32x4 (&ra)[SM], u32x4 (&rb)[SN]) __attribute__((always_inline)) {
+            const u32x4* at = smem + (s & 1) * STAGE + (lane & 31) * CH + swizzle<CH>(lane & 31, ks * 2 + (lane >> 5));
 #pragma unroll
-        for (int s = 0; s < NBUF - 1; ++s)
-            if (s < stages) fetch(s);
+            for (int j = 0; j < SM; ++j) ra[j] = at[(wm * TM + j * 32) * CH];
+#pragma unroll
+            for (int i = 0; i < SN; ++i) rb[i] = at[(BM + wn * TN + i * 32) * CH];
+        };
+        auto mma = [&](u32x4 (&ra)[SM], u32x4 (&rb)[SN]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < SN; ++i)
+#pragma unroll
+                for (int j = 0; j < SM; ++j) acc[i][j] = Num<T>::mma(rb[i], ra[j], acc[i][j]);
+        };
+        static_assert(NBUF == 2 && CH / 2 % 2 == 0, "two stages in LDS, an even number of k steps in each");
+        fetch(0);
+        if (stages > 1) {
+            fetch(1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(INSTR) : "memory");      // loads return in order: stage 0 is there
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(0, 0, a[0], b[0]);
         for (int s = 0; s < stages; ++s) {
-            // stage s has landed when at most the loads of the younger stages are still in flight (they return in order)
-            // and this wave's own reads of stage s - 1 are done
-            if (s + NBUF - 2 < stages) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF - 2) * INSTR) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();             // everybody's pieces are there, and nobody reads stage s - 1 any more
+#pragma unroll
+            for (int ks = 0; ks + 1 < CH / 2; ++ks) {
+                read(s, ks + 1, a[(ks + 1) & 1], b[(ks + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                mma(a[ks & 1], b[ks & 1]);
+            }
+            // this wave has its last operands of stage s, and its loads of stage s + 1; then everybody has
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (s + NBUF - 1 < stages) fetch(s + NBUF - 1);
-            multiply(smem + (s % NBUF) * STAGE, s + 1 < stages ? CH / 2 : last_steps);
+            if (s + 2 < stages) fetch(s + 2);
+            if (s + 1 < stages) read(s + 1, 0, a[0], b[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            mma(a[1], b[1]);
         }
     } else {
         constexpr int PIECES = STAGE / THREADS;
@@ -547,6 +578,28 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void cols_gemm_kernel(const T* __r
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
+    // 16 bits: k step ks of the 32 columns from c0 of a tile, one column per lane
+    auto columns = [&](const u32x4* tile, int ks, int c0) __attribute__((always_inline)) {
+        using S4 = __attribute__((ext_vector_type(4))) short;
+        const int row = ks * 16 + 8 * (lane >> 5) + ((lane >> 2) & 3), col = c0 + 16 * ((lane >> 4) & 1) + (lane & 3) * 4;
+        const char* at = reinterpret_cast<const char*>(tile) + (row * CP + col_swizzle<T, BC>(row, col / 8)) * 16 + (col & 4) * 2;
+        // four rows further: the same swizzle
+        const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)at);
+        const S4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)(at + 4 * CP * 16));
+        return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto read = [&](const u32x4* buf, int ks, u32x4 (&a)[SM], u32x4 (&b)[SN]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < SM; ++j) a[j] = columns(buf, ks, wm * TM + j * 32);
+#pragma unroll
+        for (int i = 0; i < SN; ++i) b[i] = columns(buf + HALF, ks, wn * TN + i * 32);
+    };
+    auto mma = [&](u32x4 (&a)[SM], u32x4 (&b)[SN]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < SN; ++i)
+#pragma unroll
+            for (int j = 0; j < SM; ++j) acc[i][j] = Num<T>::mma(b[i], a[j], acc[i][j]);
+    };
     auto multiply = [&](const u32x4* buf) __attribute__((always_inline)) {
         if constexpr (sizeof(T) == 4) {
             const float* gs = reinterpret_cast<const float*>(buf);
@@ -565,26 +618,11 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void cols_gemm_kernel(const T* __r
                     for (int j = 0; j < SM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[i], a[j], acc[i][j], 0, 0, 0);
             }
         } else {
-            using S4 = __attribute__((ext_vector_type(4))) short;
-            auto read = [&](const u32x4* tile, int ks, int c0) __attribute__((always_inline)) {
-                const int row = ks * 16 + 8 * (lane >> 5) + ((lane >> 2) & 3), col = c0 + 16 * ((lane >> 4) & 1) + (lane & 3) * 4;
-                const char* at = reinterpret_cast<const char*>(tile) + (row * CP + col_swizzle<T, BC>(row, col / 8)) * 16 + (col & 4) * 2;
-                // four rows further: the same swizzle
-                const S4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)at);
-                const S4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4*)(at + 4 * CP * 16));
-                return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            };
 #pragma unroll
             for (int ks = 0; ks < KP / 16; ++ks) {
                 u32x4 a[SM], b[SN];
-#pragma unroll
-                for (int j = 0; j < SM; ++j) a[j] = read(buf, ks, wm * TM + j * 32);
-#pragma unroll
-                for (int i = 0; i < SN; ++i) b[i] = read(buf + HALF, ks, wn * TN + i * 32);
-#pragma unroll
-                for (int i = 0; i < SN; ++i)
-#pragma unroll
-                    for (int j = 0; j < SM; ++j) acc[i][j] = Num<T>::mma(b[i], a[j], acc[i][j]);
+                read(buf, ks, a, b);
+                mma(a, b);
             }
         }
     };
@@ -605,13 +643,43 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void cols_gemm_kernel(const T* __r
                                                  (__attribute__((address_space(3))) void*)(buf + (i * WAVES + wave) * 64), 16, 0, 0);
             }
         };
-        if (stages > 0) fetch(0);
-        for (int s = 0; s < stages; ++s) {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if constexpr (sizeof(T) == 2) {                // handed over as in rows_gemm_kernel, in front of the last k step's multiplication
+            constexpr int STEPS = KP / 16;
+            u32x4 a[2][SM], b[2][SN];
+            fetch(0);
+            if (stages > 1) {
+                fetch(1);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(INSTR) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (s + 1 < stages) fetch(s + 1);
-            multiply(smem + (s % NBUF) * STAGE);
+            read(smem, 0, a[0], b[0]);
+            for (int s = 0; s < stages; ++s) {
+#pragma unroll
+                for (int ks = 0; ks + 1 < STEPS; ++ks) {
+                    read(smem + (s & 1) * STAGE, ks + 1, a[(ks + 1) & 1], b[(ks + 1) & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    mma(a[ks & 1], b[ks & 1]);
+                }
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (s + 2 < stages) fetch(s + 2);
+                if (s + 1 < stages) read(smem + ((s + 1) & 1) * STAGE, 0, a[0], b[0]);
+                __builtin_amdgcn_sched_barrier(0);
+                mma(a[1], b[1]);
+            }
+        } else {
+            fetch(0);
+            for (int s = 0; s < stages; ++s) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (s + 1 < stages) fetch(s + 1);
+                multiply(smem + (s % NBUF) * STAGE);
+            }
         }
         __syncthreads();
     } else {
@@ -1142,19 +1210,20 @@ void rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups,
     else launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
 }
 
-// The weight gradient's tiles and split: 128-column tiles, 64 where a side is that small; p in as many parts as give every CU two
-// workgroups, each at least eight stages long.
+// The weight gradient's tiles and split: 128-column tiles, 64 where a side is that small, 256 (16 bits, aligned rows) where those alone give
+// most of the CUs a tile; p in as many parts as give every CU two workgroups (one of the 256 tiles), each at least four stages long.
 struct ColsPlan {
     int bc, nt, kt, splits;
     long rows_per_split;
 };
-ColsPlan plan_cols(int64_t P, int N, int K, int groups, int dtype) {
+ColsPlan plan_cols(int64_t P, int N, int K, int groups, int dtype, bool dma) {
     ColsPlan p;
     p.bc = N > 64 && K > 64 ? 128 : 64;
+    if (dtype != 0 && dma && cdiv64(N, 256) * cdiv64(K, 256) * groups >= 192) p.bc = 256;
     p.nt = cdiv(N, p.bc);
     p.kt = cdiv(K, p.bc);
     const int64_t tiles = (int64_t)p.nt * p.kt * groups, kp = dtype == 0 ? 32 : 64;
-    int64_t splits = cdiv64(512, tiles), most = cdiv64(P, 4 * kp);
+    int64_t splits = cdiv64(p.bc == 256 ? 256 : 512, tiles), most = cdiv64(P, 4 * kp);
     if (splits > most) splits = most;
     if (splits > 512) splits = 512;
     p.rows_per_split = cdiv64(cdiv64(P, splits), kp) * kp;
@@ -1162,14 +1231,16 @@ ColsPlan plan_cols(int64_t P, int N, int K, int groups, int dtype) {
     return p;
 }
 
-template <typename T, int BC, int DMA>
+template <typename T, int BC, int WR, int WC, int DMA>
 void launch_cols_gemm(const T* G, const T* X, T* out, float* partial, long P, int N, int K, int groups, long ldg, long ldx, const ColsPlan& p,
                       hipStream_t s) {
     constexpr int KP = sizeof(T) == 4 ? 32 : 64;
     const size_t lds = (size_t)2 * 2 * KP * BC * sizeof(T);
+    auto* kernel = &cols_gemm_kernel<T, BC, WR, WC, DMA>;
+    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     const dim3 grid((unsigned)(cdiv64((int64_t)p.nt * p.kt, kXcds) * kXcds), (unsigned)groups, (unsigned)p.splits);
-    hipLaunchKernelGGL((cols_gemm_kernel<T, BC, 2, 2, DMA>), grid, dim3(256), lds, s, G, X, out, p.splits > 1 ? partial : nullptr, P, N, K, ldg,
-                       ldx, p.nt, p.kt, p.rows_per_split);
+    hipLaunchKernelGGL((cols_gemm_kernel<T, BC, WR, WC, DMA>), grid, dim3(64 * WR * WC), lds, s, G, X, out, p.splits > 1 ? partial : nullptr, P, N,
+                       K, ldg, ldx, p.nt, p.kt, p.rows_per_split);
 }
 
 SplitSum split_sum(const float* partial, void* out, int out_f32, long n, int splits) {
@@ -1177,17 +1248,23 @@ SplitSum split_sum(const float* partial, void* out, int out_f32, long n, int spl
     return SplitSum{partial, out, out_f32, splits, parts, n, (unsigned)cdiv64(n, 256 / parts)};
 }
 
-// `padded`: G's rows are followed by zeros up to whole pieces
+// `padded`: G's rows are followed by zeros up to whole pieces.  Returns the split
 template <typename T>
-void cols_gemm(const T* G, const T* X, T* out, float* partial, long P, int N, int K, int groups, long ldg, long ldx, bool padded, int dtype,
-               hipStream_t s) {
+int cols_gemm(const T* G, const T* X, T* out, float* partial, long P, int N, int K, int groups, long ldg, long ldx, bool padded, int dtype,
+              hipStream_t s) {
     constexpr size_t S = sizeof(T);
-    const ColsPlan p = plan_cols(P, N, K, groups, dtype);
     const bool dma = on16(G, ldg, S) && on16(X, ldx, S) && (long)K * S % 16 == 0 && ((long)N * S % 16 == 0 || (padded && groups == 1));
-    if (p.bc == 128 && dma) launch_cols_gemm<T, 128, 1>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
-    else if (p.bc == 128) launch_cols_gemm<T, 128, 0>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
-    else if (dma) launch_cols_gemm<T, 64, 1>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
-    else launch_cols_gemm<T, 64, 0>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    const ColsPlan p = plan_cols(P, N, K, groups, dtype, dma);
+    if constexpr (S == 2)
+        if (p.bc == 256) {
+            launch_cols_gemm<T, 256, 2, 4, 1>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+            return p.splits;
+        }
+    if (p.bc == 128 && dma) launch_cols_gemm<T, 128, 2, 2, 1>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    else if (p.bc == 128) launch_cols_gemm<T, 128, 2, 2, 0>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    else if (dma) launch_cols_gemm<T, 64, 2, 2, 1>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    else launch_cols_gemm<T, 64, 2, 2, 0>(G, X, out, partial, P, N, K, groups, ldg, ldx, p, s);
+    return p.splits;
 }
 
 // Workspace of a backward call: [dz][transposed weight][column sums][split blocks]
@@ -1196,7 +1273,6 @@ struct BwdPlan {
     int ldt, lanes, col_blocks, row_blocks;
     int64_t rows_per_block;
     size_t dz, wt, sums, split, total;
-    ColsPlan cols;
 };
 BwdPlan plan_bwd(int64_t P, int N, int K, int groups, int dtype, int act, bool want_gx, bool want_gw, bool want_gb) {
     BwdPlan b{};
@@ -1220,8 +1296,10 @@ BwdPlan plan_bwd(int64_t P, int N, int K, int groups, int dtype, int act, bool w
     b.dz = act != kActNone && (want_gx || want_gw) ? align256((size_t)P * b.ld_dz * S) : 0;
     b.wt = want_gx ? align256((size_t)groups * K * b.ldt * S) : 0;
     b.sums = want_gb ? align256((size_t)b.row_blocks * C * 4) : 0;
-    b.cols = plan_cols(P, N, K, groups, dtype);
-    b.split = want_gw && b.cols.splits > 1 ? (size_t)b.cols.splits * groups * N * K * 4 : 0;
+    if (want_gw) {           // room for either split: which tiles it is depends on the rows' alignment as well
+        const int a = plan_cols(P, N, K, groups, dtype, false).splits, c = plan_cols(P, N, K, groups, dtype, true).splits, splits = a > c ? a : c;
+        b.split = splits > 1 ? (size_t)splits * groups * N * K * 4 : 0;
+    }
     b.total = b.dz + b.wt + b.sums + b.split;
     return b;
 }
@@ -1258,11 +1336,11 @@ int launch_bwd(const T* gy, const T* x, const T* w, const void* saved, int kind,
         // the zeros behind N in dz and in wt's rows are multiplied along: whole pieces
         rows_gemm<T>(gy, wt, gx, P, K, padded && groups == 1 ? b.ldt : N, groups, ldg, b.ldt, (long)groups * K, (long)K * b.ldt, none, s);
     }
-    if (gw) cols_gemm<T>(gy, x, gw, split, P, N, K, groups, ldg, ldx, padded, dtype, s);
+    const int splits = gw ? cols_gemm<T>(gy, x, gw, split, P, N, K, groups, ldg, ldx, padded, dtype, s) : 1;
     SplitSum first{}, second{};
     first.parts = second.parts = 1;
     if (gb) first = split_sum(sums, gb, gb_f32, C, b.row_blocks);
-    if (b.split) second = split_sum(split, gw, 0, (long)groups * N * K, b.cols.splits);
+    if (splits > 1) second = split_sum(split, gw, 0, (long)groups * N * K, splits);
     if (first.blocks + second.blocks)
         hipLaunchKernelGGL(split_sum_kernel<T>, dim3(first.blocks + second.blocks), dim3(256), 0, s, first, second);
     return check_launch("linear_act_bwd");
