@@ -884,6 +884,11 @@ __global__ __launch_bounds__(256) void transpose_weight_kernel(const T* __restri
 // Results stay in registers: the lane halves of a 32 x 32 tile hold alternate groups of four columns; in 16 bits an exchange between the
 // halves makes that eight consecutive columns, so residual, z and output move as 16-byte pieces.
 // KS: k steps (two pieces each), zeros behind K; LOW: the steps that are whole in every K of this size.
+template <int E, int N>
+__device__ __forceinline__ const float (&piece(const float (&f)[N], int q))[E] {
+    return *reinterpret_cast<const float(*)[E]>(&f[q * E]);
+}
+
 template <typename T, int LOW, int KS, int THREADS>
 __global__ __launch_bounds__(THREADS, THREADS / 256) void panel_gemm_kernel(const T* __restrict__ X, const T* __restrict__ W, T* __restrict__ out, long M,
                                                                           int N, int K, int groups, long ldx, long ldw, long ldo, long wg, int pg,
@@ -969,25 +974,57 @@ __global__ __launch_bounds__(THREADS, THREADS / 256) void panel_gemm_kernel(cons
                 __builtin_amdgcn_sched_barrier(0);
                 acc = Num<T>::mma(w[ks % 4], xi[ks], acc);
             }
+            float f[16];                                        // piece q: columns 16 q + 8 half + 0..7 (16 bits), 8 q + 4 half + 0..3 (float32)
+            if constexpr (E == 8) {
 #pragma unroll
-            for (int q = 0; q < 16 / E; ++q) {                  // 16 bits: columns 16 q + 8 half + 0..7; float32: 8 q + 4 half + 0..3
-                float f[E];
-                if constexpr (E == 8) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float lower = acc[q * 8 + j], upper = acc[q * 8 + 4 + j];
-                        const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lower), __builtin_bit_cast(unsigned, upper),
-                                                                           false, false);
-                        const unsigned lo = both[0], hi = both[1];
-                        f[j] = __builtin_bit_cast(float, lo);
-                        f[4 + j] = __builtin_bit_cast(float, hi);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) f[j] = acc[q * 4 + j];
+                for (int i = 0; i < 8; ++i) {
+                    const float lower = acc[i / 4 * 8 + i % 4], upper = acc[i / 4 * 8 + 4 + i % 4];
+                    const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lower), __builtin_bit_cast(unsigned, upper), false,
+                                                                       false);
+                    const unsigned lo = both[0], hi = both[1];
+                    f[i / 4 * 8 + i % 4] = __builtin_bit_cast(float, lo);
+                    f[i / 4 * 8 + 4 + i % 4] = __builtin_bit_cast(float, hi);
                 }
-                const int valid = min(E, rows - c0 - half * E - q * 2 * E);
-                if (m < M && valid > 0) finish_piece<T>(f, add[q], orow, col0 + q * 2 * E, valid, e.act, e.slope);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) f[i] = acc[i];
+            }
+            // whole pieces, predicated by the lane's row and columns; where the columns end inside a piece, its elements one by one (a
+            // branch that is the same for all lanes, taken for the last tile of an odd width)
+            const bool mine = m < M, ragged = rows % E != 0 && c0 + 32 > rows;
+            const int left = rows - c0 - half * E;              // columns from this lane's first
+            if (e.pre) {
+#pragma unroll
+                for (int q = 0; q < 16 / E; ++q) {
+                    typename Num<T>::Pre* at = orow.pre + col0 + q * 2 * E;
+                    if (mine && left >= q * 2 * E + E) store16(at, Num<T>::pack_pre(piece<E>(f, q)));
+                    else if (ragged && mine) {
+#pragma unroll
+                        for (int i = 0; i < E; ++i)
+                            if (left > q * 2 * E + i) at[i] = Num<T>::pre(f[q * E + i]);
+                    }
+                }
+            }
+            activate<Num<T>::fast>(f, e.act, e.slope);
+            if (e.residual) {
+                const bool end = g * N + n0 + c0 + 32 > C;      // pieces that pass the row's end were fetched from in front of it
+#pragma unroll
+                for (int q = 0; q < 16 / E; ++q) {
+                    float r[E];
+                    Num<T>::unpack(end ? tail_fixed<T>(add[q], min(col0 + q * 2 * E, C - 1), C) : add[q], r);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) f[q * E + i] += r[i];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 16 / E; ++q) {
+                T* at = orow.out + col0 + q * 2 * E;
+                if (mine && left >= q * 2 * E + E) store16(at, Num<T>::pack(piece<E>(f, q)));
+                else if (ragged && mine) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+                        if (left > q * 2 * E + i) at[i] = (T)f[q * E + i];
+                }
             }
         }
     };

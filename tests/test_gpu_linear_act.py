@@ -152,6 +152,26 @@ def test_values_and_gradients(ops, P, K, N, groups, t):
     _check(_run(ops, x, w, b, r, gy, act, 0.01, groups), _expect(x, w, b, r, gy, act, 0.01, groups))
 
 
+_MANY = [
+    # P, K, N, groups: the weight in LDS (every register size, panels of several groups and of parts of one group, odd widths) and the largest tiles
+    (16384, 9, 5, 1), (16400, 44, 44, 6), (16385, 20, 33, 3), (16390, 132, 72, 1), (20000, 100, 529, 1), (16447, 200, 264, 1), (16384, 264, 96, 1), (16500, 266, 700, 1),
+    (16401, 393, 40, 1), (16384, 528, 132, 1), (33000, 17, 1, 40), (17000, 67, 131, 2), (8200, 200, 4104, 1), (260, 4104, 3080, 1),
+]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("P,K,N,groups", _MANY)
+def test_many_rows_and_large_weights(ops, P, K, N, groups, t):
+    i = _MANY.index((P, K, N, groups))
+    bias, residual = i % 3 != 1, i % 2 == 0
+    act = ["gelu", "none", "gelu"][(i + 1) % 3]
+    x, w, b, r, gy = _inputs(P, K, N, groups, t, 300 + i, bias=bias, residual=residual)
+    _check(_run(ops, x, w, b, r, gy, act, 0.01, groups), _expect(x, w, b, r, gy, act, 0.01, groups))
+    with torch.no_grad():
+        y = ops.linear_act(x, w, b, r, "none", groups=groups)
+    _check({"y": y}, _expect(x, w, b, r, None, "none", 0.01, groups))
+
+
 @pytest.mark.parametrize("t", TYPES, ids=str)
 @pytest.mark.parametrize("act,slope", [("relu", 0.01), ("leakyrelu", 0.01), ("leakyrelu", 0.0), ("leakyrelu", -0.5), ("leakyrelu", 1.5), ("hswish", 0.01), ("none", 0.0)])
 @pytest.mark.parametrize("P,K,N,groups,residual", [(70, 12, 9, 1, False), (70, 12, 9, 1, True), (300, 16, 72, 2, False), (6, 200, 136, 1, True), (260, 256, 256, 1, False)])
