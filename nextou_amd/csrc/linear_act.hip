@@ -1260,7 +1260,8 @@ ColsPlan plan_cols(int64_t P, int N, int K, int groups, int dtype, bool dma) {
     p.nt = cdiv(N, p.bc);
     p.kt = cdiv(K, p.bc);
     const int64_t tiles = (int64_t)p.nt * p.kt * groups, kp = dtype == 0 ? 32 : 64;
-    int64_t splits = cdiv64(p.bc == 256 ? 256 : 512, tiles), most = cdiv64(P, 4 * kp);
+    int64_t splits = (p.bc == 256 ? 256 : 512) / tiles, most = cdiv64(P, 4 * kp);      // rounded down: one workgroup too many is a second round
+    if (splits < 1) splits = 1;
     if (splits > most) splits = most;
     if (splits > 512) splits = 512;
     p.rows_per_split = cdiv64(cdiv64(P, splits), kp) * kp;

@@ -1854,20 +1854,22 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         raise ValueError("linear_act: bias %s for %d output channels" % (tuple(bias.shape), weight.shape[0]))
     if residual is not None and tuple(residual.shape) != tuple(x.shape[:-1]) + (weight.shape[0],):
         raise ValueError("linear_act: residual %s for an output of %s" % (tuple(residual.shape), tuple(x.shape[:-1]) + (weight.shape[0],)))
-    given = [t for t in (x, weight, bias, residual) if t is not None]
-    if any(t.device != x.device for t in given):
-        raise ValueError("linear_act: tensors on %s" % ", ".join(sorted({str(t.device) for t in given})))
-    if x.is_cuda and torch.is_autocast_enabled("cuda") and all(t.dtype in _LINEAR_TYPES for t in given):
+    dev = x.device
+    if weight.device != dev or (bias is not None and bias.device != dev) or (residual is not None and residual.device != dev):
+        raise ValueError("linear_act: tensors on %s" % ", ".join(sorted({str(t.device) for t in (x, weight, bias, residual) if t is not None})))
+    if x.is_cuda and torch.is_autocast_enabled("cuda") and all(t is None or t.dtype in _LINEAR_TYPES for t in (x, weight, bias, residual)):
         dt = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dt), weight.to(dt)
         bias = bias if bias is None or bias.dtype == torch.float32 else bias.to(dt)
         residual = None if residual is None else residual.to(dt)
-    if x.dtype not in _LINEAR_TYPES or weight.dtype != x.dtype or (residual is not None and residual.dtype != x.dtype) or \
-            (bias is not None and bias.dtype not in (x.dtype, torch.float32)):
+    dt = x.dtype
+    if dt not in _LINEAR_TYPES or weight.dtype != dt or (residual is not None and residual.dtype != dt) or \
+            (bias is not None and bias.dtype != dt and bias.dtype != torch.float32):
         raise TypeError("linear_act: float32, bfloat16 or float16 tensors of one type (a float32 bias apart), got %s" %
-                        ", ".join(str(t.dtype) for t in given))
+                        ", ".join(str(t.dtype) for t in (x, weight, bias, residual) if t is not None))
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    training = torch.is_grad_enabled() and any(t.requires_grad for t in given)
+    training = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                            (residual is not None and residual.requires_grad))
     if not training and x.numel():
         y, _ = _backend_for(x).linear_act_fwd(_as_rows(x), weight.contiguous(), bias, None if residual is None else _as_rows(residual),
                                               _LINEAR_ACTS[act], float(negative_slope), groups, False)

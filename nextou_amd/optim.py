@@ -83,7 +83,7 @@ _NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _NORM_CODES = {math.inf: 0, 1.0: 1, 2.0: 2}
 _LAST = {4: torch.channels_last, 5: torch.channels_last_3d}
 _DTYPE, _DEVICE = operator.attrgetter("dtype"), operator.attrgetter("device")
-_GRAD, _LAYOUT = operator.attrgetter("grad"), operator.attrgetter("layout")
+_GRAD = operator.attrgetter("grad")
 
 
 def _norm_code(norm_type) -> int:
@@ -99,14 +99,17 @@ def _flat_run(t: torch.Tensor) -> bool:
 
 def _norm_rows(tensors: List[torch.Tensor], in_place: bool):
     """(host table, [(tensor, its dense copy)]) of the tensors that have elements; everything the kernels do not take is refused here."""
-    if set(map(_LAYOUT, tensors)) == {torch.strided} and all(map(torch.Tensor.is_contiguous, tensors)):
+    try:
         # the usual list, attribute by attribute (a few hundred tensors: the loop below costs more than the kernels)
-        counts, types = list(map(torch.Tensor.numel, tensors)), list(map(_NORM_TYPES.get, map(_DTYPE, tensors)))
-        if None not in types and 0 not in counts and len(set(map(_DEVICE, tensors))) == 1:
-            vals = array.array("q", bytes(24 * len(tensors)))
-            vals[0::3] = array.array("q", map(torch.Tensor.data_ptr, tensors))
-            vals[1::3], vals[2::3] = array.array("q", counts), array.array("q", types)
-            return vals, []
+        if all(map(torch.Tensor.is_contiguous, tensors)):
+            counts, types = list(map(torch.Tensor.numel, tensors)), list(map(_NORM_TYPES.get, map(_DTYPE, tensors)))
+            if None not in types and 0 not in counts and len(set(map(_DEVICE, tensors))) == 1:
+                vals = array.array("q", bytes(24 * len(tensors)))
+                vals[0::3] = array.array("q", map(torch.Tensor.data_ptr, tensors))      # (a tensor without storage raises here)
+                vals[1::3], vals[2::3] = array.array("q", counts), array.array("q", types)
+                return vals, []
+    except (RuntimeError, NotImplementedError):
+        pass
     device, vals, copies = tensors[0].device, array.array("q"), []
     for t in tensors:
         code = _NORM_TYPES.get(t.dtype)
