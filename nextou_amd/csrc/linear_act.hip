@@ -13,7 +13,6 @@ using bf16_t = __bf16;
 using f16_t = _Float16;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
-using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
 
 enum Act { kActNone = 0, kActRelu = 1, kActLeaky = 2, kActGelu = 3, kActHardswish = 4 };
 
@@ -46,7 +45,7 @@ __device__ __forceinline__ void activate(float (&f)[E], int act, float slope) {
 #pragma unroll
         for (int i = 0; i < E; ++i) f[i] = f[i] <= 0.f ? 0.f : f[i];             // (NaN stays NaN)
     } else if (act == kActLeaky) {
-        if (slope >= 0.f && slope <= 1.f) {
+        if (slope > 0.f && slope <= 1.f) {
 #pragma unroll
             for (int i = 0; i < E; ++i) f[i] = fmaxf(f[i], f[i] * slope);
         } else {
@@ -214,11 +213,11 @@ __device__ __forceinline__ u32x4 tail_fixed(u32x4 v, long c, long C) {
 //
 // A workgroup of WR x WC waves computes BM x BN outputs; a wave its (BM / WR) x (BN / WC) block out of 32 x 32 matrix-unit tiles, n in the
 // tile's rows: a lane ends up with four consecutive n of one m.  k advances in stages of CH 16-byte pieces per row (CH = 8: 64 sixteen-bit
-// or 32 float values), kept in LDS as [row][piece] with the piece index XORed by the row, so that the sixteen lanes that are served
+// or 32 float values), two stages kept in LDS as [row][piece] with the piece index XORed by the row, so that the sixteen lanes that are served
 // together (16 rows, one piece) fall on all sixteen 16-byte columns of the 64 banks.  In float32 a piece feeds four matrix instructions, in 16 bits one: the same addresses.
 //
 // DMA = 1: every row starts on 16 bytes and K is a whole number of pieces; stages go from memory to LDS without registers
-// (global_load_lds), NBUF - 1 stages ahead, one barrier a stage.  Rows behind the end are read from the last row (their outputs are not
+// (global_load_lds), one barrier a stage.  Rows behind the end are read from the last row (their outputs are not
 // stored), pieces behind K from sixteen zero bytes.
 // DMA = 0: any alignment and any K; a stage waits in registers while the previous one is multiplied.
 //
@@ -236,11 +235,8 @@ struct Epilogue {
     float slope;
 };
 
-template <int CH>
-__device__ __forceinline__ int swizzle(int row, int piece) {
-    if constexpr (CH == 8) return piece ^ ((row >> 1) & 7);
-    else return piece ^ ((row >> 2) & 3);
-}
+constexpr int CH = 8, NBUF = 2;     // pieces of a row in a stage, stages in LDS
+__device__ __forceinline__ int swizzle(int row, int piece) { return piece ^ ((row >> 1) & 7); }
 
 // LDS written by a wave is read by the same wave's other lanes behind this (its LDS instructions run in order)
 __device__ __forceinline__ void wave_sync() {
@@ -336,7 +332,7 @@ __device__ __forceinline__ void load_bias(float (&b)[Num<T>::E], const Epilogue&
     }
 }
 
-template <typename T, int BM, int BN, int WR, int WC, int CH, int NBUF, int DMA>
+template <typename T, int BM, int BN, int WR, int WC, int DMA>
 __global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 : 2) void rows_gemm_kernel(
     const T* __restrict__ A, const T* __restrict__ B, T* __restrict__ out, long M, int N, int K, long lda, long ldb, long ldo, long bg, int mt, int nt,
     Epilogue e) {
@@ -372,9 +368,9 @@ __global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 
             if (ks < steps) {
                 u32x4 a[SM], b[SN];
 #pragma unroll
-                for (int j = 0; j < SM; ++j) a[j] = as[(j * 32 + r32) * CH + swizzle<CH>(r32, ks * 2 + half)];
+                for (int j = 0; j < SM; ++j) a[j] = as[(j * 32 + r32) * CH + swizzle(r32, ks * 2 + half)];
 #pragma unroll
-                for (int i = 0; i < SN; ++i) b[i] = bs[(i * 32 + r32) * CH + swizzle<CH>(r32, ks * 2 + half)];
+                for (int i = 0; i < SN; ++i) b[i] = bs[(i * 32 + r32) * CH + swizzle(r32, ks * 2 + half)];
 #pragma unroll
                 for (int i = 0; i < SN; ++i)
 #pragma unroll
@@ -393,13 +389,13 @@ __global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 
         for (int i = 0; i < INSTR; ++i) {
             const int row = (i * WAVES + wave) * RPI + lane / CH;          // INSTR x WAVES x RPI rows, A rows below BM
             const int in = row < BM ? row : row - BM;
-            piece[i] = swizzle<CH>(in, lane % CH);
+            piece[i] = swizzle(in, lane % CH);
             src[i] = row < BM ? reinterpret_cast<const char*>(A + min(m0 + in, M - 1) * lda)
                               : reinterpret_cast<const char*>(B + (long)min(n0 + in, N - 1) * ldb);
         }
         const int pieces = K / E;
         auto fetch = [&](int s) __attribute__((always_inline)) {
-            u32x4* buf = smem + (s % NBUF) * STAGE;
+            u32x4* buf = smem + (s & 1) * STAGE;
             const bool whole = (s + 1) * CH <= pieces;
 #pragma unroll
             for (int i = 0; i < INSTR; ++i) {
@@ -415,7 +411,7 @@ __global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 
         // just read is free for the stage after the next, and the first operands of the next stage arrive behind the multiplication.
         u32x4 a[2][SM], b[2][SN];
         auto read = [&](int s, int ks, u32x4 (&ra)[SM], u32x4 (&rb)[SN]) __attribute__((always_inline)) {
-            const u32x4* at = smem + (s & 1) * STAGE + (lane & 31) * CH + swizzle<CH>(lane & 31, ks * 2 + (lane >> 5));
+            const u32x4* at = smem + (s & 1) * STAGE + (lane & 31) * CH + swizzle(lane & 31, ks * 2 + (lane >> 5));
 #pragma unroll
             for (int j = 0; j < SM; ++j) ra[j] = at[(wm * TM + j * 32) * CH];
 #pragma unroll
@@ -427,7 +423,6 @@ __global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 
 #pragma unroll
                 for (int j = 0; j < SM; ++j) acc[i][j] = Num<T>::mma(rb[i], ra[j], acc[i][j]);
         };
-        static_assert(NBUF == 2 && CH / 2 % 2 == 0, "two stages in LDS, an even number of k steps in each");
         fetch(0);
         if (stages > 1) {
             fetch(1);
@@ -473,7 +468,7 @@ __global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
                 const int row = (i * THREADS + tid) / CH;
-                buf[row * CH + swizzle<CH>(row < BM ? row : row - BM, pc)] = whole ? held[i] : tail_fixed<T>(held[i], (long)s * KE + pc * E, K);
+                buf[row * CH + swizzle(row < BM ? row : row - BM, pc)] = whole ? held[i] : tail_fixed<T>(held[i], (long)s * KE + pc * E, K);
             }
         };
         fetch(0);
@@ -523,16 +518,16 @@ __global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 
     }
 }
 
-template <typename T, int BM, int BN, int WR, int WC, int CH, int NBUF, int DMA>
+template <typename T, int BM, int BN, int WR, int WC, int DMA>
 void launch_rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
                       hipStream_t s) {
     const int mt = (int)cdiv64(M, BM), nt = cdiv(N, BN);
     const size_t lds = (size_t)(BM + BN) * CH * 16 * NBUF;
-    auto* kernel = &rows_gemm_kernel<T, BM, BN, WR, WC, CH, NBUF, DMA>;
+    auto* kernel = &rows_gemm_kernel<T, BM, BN, WR, WC, DMA>;
     if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     const int64_t items = (int64_t)mt * nt;
     const dim3 grid((unsigned)(cdiv64(items, kXcds) * kXcds), (unsigned)groups);
-    hipLaunchKernelGGL((rows_gemm_kernel<T, BM, BN, WR, WC, CH, NBUF, DMA>), grid, dim3(64 * WR * WC), lds, s, A, B, out, M, N, K, lda, ldb, ldo, bg,
+    hipLaunchKernelGGL((rows_gemm_kernel<T, BM, BN, WR, WC, DMA>), grid, dim3(64 * WR * WC), lds, s, A, B, out, M, N, K, lda, ldb, ldo, bg,
                        mt, nt, e);
 }
 
@@ -556,7 +551,7 @@ template <typename T, int BC, int WR, int WC, int DMA>
 __global__ __launch_bounds__(64 * WR * WC, 2) void cols_gemm_kernel(const T* __restrict__ G, const T* __restrict__ X, T* __restrict__ out,
                                                                     float* __restrict__ partial, long P, int N, int K, long ldg, long ldx, int nt,
                                                                     int kt, long rows_per_split) {
-    constexpr int E = Num<T>::E, CP = BC / E, THREADS = 64 * WR * WC, WAVES = WR * WC, NBUF = 2;
+    constexpr int E = Num<T>::E, CP = BC / E, THREADS = 64 * WR * WC, WAVES = WR * WC;
     constexpr int KP = sizeof(T) == 4 ? 32 : 64, HALF = KP * CP, STAGE = 2 * HALF;       // pieces; G's tile, then X's
     constexpr int TM = BC / WR, TN = BC / WC, SM = TM / 32, SN = TN / 32;
     extern __shared__ u32x4 smem[];
@@ -630,7 +625,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void cols_gemm_kernel(const T* __r
     if constexpr (DMA) {
         constexpr int INSTR = STAGE / 64 / WAVES;
         auto fetch = [&](int s) __attribute__((always_inline)) {
-            u32x4* buf = smem + (s % NBUF) * STAGE;
+            u32x4* buf = smem + (s & 1) * STAGE;
 #pragma unroll
             for (int i = 0; i < INSTR; ++i) {
                 const int q = (i * WAVES + wave) * 64 + lane, in = q < HALF ? q : q - HALF;
@@ -889,11 +884,13 @@ __device__ __forceinline__ const float (&piece(const float (&f)[N], int q))[E] {
     return *reinterpret_cast<const float(*)[E]>(&f[q * E]);
 }
 
-template <typename T, int LOW, int KS, int THREADS>
-__global__ __launch_bounds__(THREADS, THREADS / 256) void panel_gemm_kernel(const T* __restrict__ X, const T* __restrict__ W, T* __restrict__ out, long M,
+constexpr int kPanelThreads = 512;                              // two waves a SIMD, 256 registers each
+
+template <typename T, int LOW, int KS>
+__global__ __launch_bounds__(kPanelThreads, 2) void panel_gemm_kernel(const T* __restrict__ X, const T* __restrict__ W, T* __restrict__ out, long M,
                                                                           int N, int K, int groups, long ldx, long ldw, long ldo, long wg, int pg,
                                                                           int pn, int parts, Epilogue e) {
-    constexpr int E = Num<T>::E, WAVES = THREADS / 64, PITCH = 2 * KS + 1;
+    constexpr int E = Num<T>::E, THREADS = kPanelThreads, WAVES = THREADS / 64, PITCH = 2 * KS + 1;
     extern __shared__ u32x4 smem[];
     const int npg = (N + pn - 1) / pn;                          // panels per group (1 when a panel holds whole groups)
     const int g0 = (int)blockIdx.y / npg * pg, g1 = min(groups, g0 + pg);
@@ -934,13 +931,11 @@ __global__ __launch_bounds__(THREADS, THREADS / 256) void panel_gemm_kernel(cons
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) x[ks] = ks < LOW ? load16(at + half * E + ks * 2 * E) : load_tail(at, (ks * 2 + half) * E, K);
     };
-    constexpr bool EARLY = KS <= 17;                            // registers for the next item's x beside this one's
     const long items = tiles * per_row, stride = (long)gridDim.x * WAVES, first = (long)blockIdx.x * WAVES + wave;
-    u32x4 x[EARLY ? 2 : 1][KS];
-    if (EARLY && first < items) fetch(first, x[0]);
+    u32x4 x[2][KS];                                             // this item's x and the next one's
+    if (first < items) fetch(first, x[0]);
     auto one = [&](long item, u32x4 (&xi)[KS], u32x4 (&xn)[KS]) __attribute__((always_inline)) {
-        if (EARLY) fetch(min(item + stride, items - 1), xn);
-        else fetch(item, xi);
+        fetch(min(item + stride, items - 1), xn);
         if (K != 2 * KS * E) {                                  // KS is the next size above: zeros behind K
 #pragma unroll
             for (int ks = LOW; ks < KS; ++ks) xi[ks] = tail_fixed<T>(xi[ks], (ks * 2 + half) * E, K);
@@ -1028,18 +1023,13 @@ __global__ __launch_bounds__(THREADS, THREADS / 256) void panel_gemm_kernel(cons
             }
         }
     };
-    if constexpr (EARLY) {
-        for (long item = first; item < items; item += 2 * stride) {
-            one(item, x[0], x[1]);
-            if (item + stride < items) one(item + stride, x[1], x[0]);
-        }
-    } else {
-        for (long item = first; item < items; item += stride) one(item, x[0], x[0]);
+    for (long item = first; item < items; item += 2 * stride) {
+        one(item, x[0], x[1]);
+        if (item + stride < items) one(item + stride, x[1], x[0]);
     }
 }
 
 constexpr int kPanelLds = 160 * 1024;
-constexpr int panel_threads(int ks) { return ks <= 3 ? 1024 : 512; }      // 128 or 256 registers
 
 // A panel for these sizes; 0 columns: the rows do not fit the registers
 struct PanelPlan {
@@ -1049,7 +1039,7 @@ struct PanelPlan {
 PanelPlan plan_panel(int N, int K, int groups, size_t S) {
     PanelPlan p{};
     const int E = (int)(16 / S), steps = cdiv(K, 2 * E);
-    static const int sizes[] = {3, 6, 9, 13, 17, 25, 34};
+    static const int sizes[] = {3, 6, 9, 13, 17};
     for (int ks : sizes)
         if (!p.ks && steps <= ks) p.ks = ks;
     if (K < E || groups * N < E) p.ks = 0;
@@ -1076,10 +1066,10 @@ PanelPlan plan_panel(int N, int K, int groups, size_t S) {
 template <typename T, int LOW, int KS>
 void launch_panel(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
                   const PanelPlan& p, hipStream_t s) {
-    constexpr int THREADS = panel_threads(KS);
-    auto* kernel = &panel_gemm_kernel<T, LOW, KS, THREADS>;
+    constexpr int THREADS = kPanelThreads;
+    auto* kernel = &panel_gemm_kernel<T, LOW, KS>;
     if (p.lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.lds);
-    const int per_cu = p.lds <= kPanelLds / 2 && THREADS <= 512 ? 2 : 1;
+    const int per_cu = p.lds <= kPanelLds / 2 ? 2 : 1;
     int64_t wgs = cdiv(256 * per_cu, p.panels);
     if (wgs > cdiv64(M, THREADS / 2)) wgs = cdiv64(M, THREADS / 2);
     // 32 rows are a large item for a wave that gets one or two of them: the columns in up to four parts, where that evens the waves out
@@ -1087,7 +1077,7 @@ void launch_panel(const T* A, const T* B, T* out, long M, int N, int K, int grou
     int parts = 1;
     for (int q = 2; q <= 4 && q * 3 <= cdiv(p.pn, 32); ++q)
         if (cdiv64(items * q, waves) * parts < cdiv64(items * parts, waves) * q) parts = q;
-    hipLaunchKernelGGL((panel_gemm_kernel<T, LOW, KS, THREADS>), dim3((unsigned)wgs, (unsigned)p.panels), dim3(THREADS), p.lds, s, A, B, out, M, N,
+    hipLaunchKernelGGL((panel_gemm_kernel<T, LOW, KS>), dim3((unsigned)wgs, (unsigned)p.panels), dim3(THREADS), p.lds, s, A, B, out, M, N,
                        K, groups, lda, ldb, ldo, bg, p.pg, p.pn, parts, e);
 }
 
@@ -1099,9 +1089,7 @@ void panel_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups
         case 6: return launch_panel<T, 3, 6>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
         case 9: return launch_panel<T, 6, 9>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
         case 13: return launch_panel<T, 9, 13>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
-        case 17: return launch_panel<T, 13, 17>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
-        case 25: return launch_panel<T, 17, 25>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
-        default: return launch_panel<T, 25, 34>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
+        default: return launch_panel<T, 13, 17>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
     }
 }
 
@@ -1161,13 +1149,13 @@ __global__ __launch_bounds__(512) void few_rows_kernel(const T* __restrict__ X, 
         u32x4 *wt = turn[wave][0], *xt = turn[wave][1];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            wt[(u * 8 + r8) * 8 + swizzle<8>(u * 8 + r8, p8)] = wb[u];
-            xt[(u * 8 + r8) * 8 + swizzle<8>(u * 8 + r8, p8)] = xb[u];
+            wt[(u * 8 + r8) * 8 + swizzle(u * 8 + r8, p8)] = wb[u];
+            xt[(u * 8 + r8) * 8 + swizzle(u * 8 + r8, p8)] = xb[u];
         }
         wave_sync();
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            acc = Num<T>::mma(wt[r32 * 8 + swizzle<8>(r32, u * 2 + half)], xt[r32 * 8 + swizzle<8>(r32, u * 2 + half)], acc);
+            acc = Num<T>::mma(wt[r32 * 8 + swizzle(r32, u * 2 + half)], xt[r32 * 8 + swizzle(r32, u * 2 + half)], acc);
         wave_sync();
     };
     for (int r = 0;;) {
@@ -1212,9 +1200,17 @@ void launch_few_rows(const T* A, const T* B, T* out, long M, int N, int K, int g
 size_t elem_bytes(int dtype) { return dtype == 0 ? 4 : 2; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-constexpr long kPanelRows = 16384;
-
-constexpr long kFewTiles = 128;
+// The panel kernel from 65536 rows on: then each of its 2048 waves has 32 rows.  Panel against tiles, us: 65536 rows bfloat16 132 -> 132 15.5 / 27.8,
+// 264 -> 528 48 / 69; 172032 rows 132 -> 528 91 / 164, float32 252 / 467; fewer rows leave waves idle, 21504 rows 132 -> 264 17.4 / 16.0, float32
+// 132 -> 132 34 / 20.  Rows of more than 17 k steps leave no registers for the next rows: 172032 rows 384 -> 384 132 / 117, 400 -> 1600 593 / 484.
+constexpr long kPanelRows = 65536;
+// k split over the waves where fewer than 64 tiles of 64 x 64 would be there, and up to 160 with rows of 4 KB and more.  Split against tiles, us:
+// bfloat16 336 rows 528 -> 528 5.9 / 7.0, 1000 rows 132 -> 132 5.0 / 6.2, 256 rows 2048 -> 2048 14.0 / 19.7; 700 rows 528 -> 528 10.9 / 7.3,
+// 512 rows 2048 -> 2048 25.5 / 20.3.  32 rows fill no tile, whatever their number of columns: 8192 -> 2048 15 / 66.
+bool few_rows(long M, int N, int K, int groups, size_t S) {
+    const long tiles = cdiv64(M, 64) * cdiv(N, 64) * groups;
+    return K >= (int)(16 / S) && (M <= 32 || tiles < 64 || (tiles <= 160 && (long)K * (long)S >= 4096));
+}
 
 // Rounds of the CUs that square tiles of three sizes need, in units of a 64 x 64 tile's matrix work; what a CU holds at a time is one 256, two
 // 128 or four 64 tiles.  Weighted by what they reach when they fill the card (16384 x 2048 -> 8192 in bfloat16: 1030, 900, 620 TFLOP/s).
@@ -1235,16 +1231,16 @@ void rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups,
         panel_gemm<T>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
         return;
     }
-    if (K >= Num<T>::E && (M <= 32 || cdiv64(M, 64) * cdiv(N, 64) * groups < kFewTiles)) {
+    if (few_rows(M, N, K, groups, S)) {
         launch_few_rows<T>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
         return;
     }
     const int tile = tile_size(M, N, groups, dma);
-    if (tile == 256) launch_rows_gemm<T, 256, 256, 2, 4, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else if (dma && tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else if (dma) launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else if (tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else launch_rows_gemm<T, 64, 64, 2, 2, 8, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    if (tile == 256) launch_rows_gemm<T, 256, 256, 2, 4, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else if (dma && tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else if (dma) launch_rows_gemm<T, 64, 64, 2, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else if (tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    else launch_rows_gemm<T, 64, 64, 2, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
 }
 
 // The weight gradient's tiles and split: 128-column tiles, 64 where a side is that small, 256 (16 bits, aligned rows) where those alone give
@@ -1388,6 +1384,10 @@ int check_sizes(const char* who, int64_t P, int N, int K, int groups, int dtype,
     NEXTOU_REQUIRE(P > 0 && P <= (1ll << 36) && N > 0 && K > 0 && groups > 0 && groups <= 65535 && (int64_t)groups * N <= (1ll << 21) &&
                        (int64_t)groups * K <= (1ll << 21) && cdiv64(P, 64) * cdiv(N > K ? N : K, 64) < (1ll << 31),
                    "%s: bad sizes (P %lld, N %d, K %d, groups %d)", who, (long long)P, N, K, groups);
+    // Rows narrower than a piece go through 64-row tiles however many there are; a launch takes fewer than 2^32 threads
+    const int E = dtype == 0 ? 4 : 8;
+    NEXTOU_REQUIRE((N >= E && K >= E) || cdiv64(P, 64) * cdiv(N > K ? N : K, 64) < (1ll << 24),
+                   "%s: too many rows of fewer than 16 bytes (P %lld, N %d, K %d)", who, (long long)P, N, K);
     NEXTOU_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d", who, dtype);
     NEXTOU_REQUIRE(act >= 0 && act <= 4, "%s: activation %d", who, act);
     return 0;

@@ -154,8 +154,9 @@ def test_values_and_gradients(ops, P, K, N, groups, t):
 
 _MANY = [
     # P, K, N, groups: the weight in LDS (every register size, panels of several groups and of parts of one group, odd widths) and the largest tiles
-    (16384, 9, 5, 1), (16400, 44, 44, 6), (16385, 20, 33, 3), (16390, 132, 72, 1), (20000, 100, 529, 1), (16447, 200, 264, 1), (16384, 264, 96, 1), (16500, 266, 700, 1),
-    (16401, 393, 40, 1), (16384, 528, 132, 1), (33000, 17, 1, 40), (17000, 67, 131, 2), (8200, 200, 4104, 1), (260, 4104, 3080, 1),
+    (65536, 9, 5, 1), (65552, 44, 44, 6), (65537, 20, 33, 3), (65542, 132, 72, 1), (70000, 100, 529, 1), (65599, 200, 264, 1), (65536, 264, 96, 1),
+    (65550, 266, 700, 1), (65553, 393, 40, 1), (65536, 528, 132, 1), (66000, 17, 1, 40), (68000, 67, 131, 2), (20000, 44, 44, 6), (16385, 132, 72, 1),
+    (8200, 200, 4104, 1), (260, 4104, 3080, 1),
 ]
 
 
@@ -267,6 +268,16 @@ def test_non_finite_values_stay_in_their_rows(ops, t):
         assert bool(torch.isnan(got["gx"][4]).all()) and not bool(torch.isnan(got["gx"][[i for i in range(P) if i != 4]]).any())
         assert bool(torch.isnan(got["gw"][0]).all()) and not bool(torch.isnan(got["gw"][1:]).any())
         assert bool(torch.isnan(got["gb"][0])) and not bool(torch.isnan(got["gb"][1:]).any())
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("slope", [0.0, 0.01, 1.0, 1.5, -0.5])
+def test_leaky_relu_of_infinities(ops, slope, t):
+    # one column of ones: z is x, exactly
+    x = torch.tensor([[float("inf")], [float("-inf")], [float("nan")], [0.0], [-2.0], [2.0]], device="cuda", dtype=t)
+    with torch.no_grad():
+        y = ops.linear_act(x, torch.ones(8, 1, device="cuda", dtype=t), None, None, "leakyrelu", slope)
+    torch.testing.assert_close(y, torch.nn.functional.leaky_relu(x, slope).expand(-1, 8), rtol=0, atol=0, equal_nan=True)
 
 
 def test_small_positive_values_keep_their_sign(ops):

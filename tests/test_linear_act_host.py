@@ -112,6 +112,7 @@ def test_c_entries_check_their_arguments():
     assert fwd(P=0) == -1 and fwd(N=0) == -1 and fwd(K=-1) == -1 and fwd(g=0) == -1 and fwd(dt=3) == -1 and fwd(act=5) == -1
     assert fwd(N=4, ldy=3) == -1 and b"stride" in L.nextou_last_error()
     assert fwd(ldx=-1) == -1 and fwd(g=70000) == -1
+    assert fwd(P=1 << 30) == -1 and b"16 bytes" in L.nextou_last_error()
     bwd = lambda **k: L.nextou_linear_act_bwd(*[{**dict(gy=16, x=16, w=16, sv=None, kind=0, gx=16, gw=None, gb=None, ws=None, wsb=0, P=1, N=1,  # noqa: E731
                                                         K=1, g=1, ldg=1, ldx=1, dt=0, gbf=0, act=0, s=0.0, st=None), **k}[i] for i in
                                                 "gy x w sv kind gx gw gb ws wsb P N K g ldg ldx dt gbf act s st".split()])
@@ -120,6 +121,8 @@ def test_c_entries_check_their_arguments():
     assert bwd(act=2, kind=2, sv=16, s=-0.5) == -1
     assert bwd(act=3, kind=1, sv=16) == -2 and b"workspace" in L.nextou_last_error()
     assert L.nextou_linear_act_bwd_workspace(4, 4, 4, 1, 9, 0, 1, 1, 1, ctypes.byref(n)) == -1
+    assert L.nextou_linear_act_bwd_workspace(1 << 30, 8, 7, 1, 1, 0, 1, 1, 1, ctypes.byref(n)) == -1
+    assert L.nextou_linear_act_bwd_workspace(1 << 30, 8, 8, 1, 1, 0, 1, 1, 1, ctypes.byref(n)) == 0
 
     assert L.nextou_multi_norm_workspace(0, ctypes.byref(n)) == -1
     assert L.nextou_multi_norm_workspace(3, ctypes.byref(n)) == 0 and n.value >= 8
