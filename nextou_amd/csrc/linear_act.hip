@@ -777,20 +777,63 @@ __global__ __launch_bounds__(256) void split_sum_kernel(SplitSum first, SplitSum
     else static_cast<T*>(a.out)[i] = (T)t;
 }
 
-// ---- the activation's gradient and the column sums ------------------------------------------------------------------------------------
+// ---- the backward's preparation: the activation's gradient with the column sums, and the transposed weight ----------------------------------
+// w (groups * N, K) -> wt (groups * K, ldt >= N), columns behind N zero: the data gradient's second operand with n contiguous
+template <typename T>
+__device__ __forceinline__ void transpose_weight(T (&tile)[64][66], const T* __restrict__ w, T* __restrict__ wt, int N, int K, int ldt, unsigned block) {
+    const int nt = (ldt + 63) / 64, kt = (K + 63) / 64;
+    const int n0 = (int)(block % nt) * 64, k0 = (int)(block / nt % kt) * 64;
+    const long g = block / nt / kt;
+    w += g * N * K;
+    wt += g * K * ldt;
+    constexpr int E = Num<T>::E, LPR = 64 / E;
+#pragma unroll
+    for (int j = 0; j < 64 * LPR / 256; ++j) {
+        const int i = j * 256 + threadIdx.x, r = i / LPR, c = i % LPR * E;
+        T v[E];
+        u32x4 piece{0, 0, 0, 0};
+        if (n0 + r < N && k0 + c < K) piece = load_piece(w + (long)(n0 + r) * K, k0 + c, K);
+        __builtin_memcpy(v, &piece, 16);
+#pragma unroll
+        for (int q = 0; q < E; ++q) tile[r][c + q] = v[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 64 * LPR / 256; ++j) {
+        const int i = j * 256 + threadIdx.x, r = i / LPR, c = i % LPR * E;
+        if (k0 + r >= K || n0 + c >= ldt) continue;             // ldt is a whole number of pieces
+        T v[E];
+        u32x4 piece;
+#pragma unroll
+        for (int q = 0; q < E; ++q) v[q] = tile[c + q][r];
+        __builtin_memcpy(&piece, v, 16);
+        store16(wt + (long)(k0 + r) * ldt + n0 + c, piece);
+    }
+}
+
 // dz = gy act'(saved) as dense rows of ld_dz columns (a multiple of 16 bytes, so that both products fetch it without registers; the columns
 // behind C are zeros), and per-workgroup column sums of the unrounded dz.  A workgroup holds `lanes` 16-byte pieces of a row and 256 / lanes
-// rows at a time; blockIdx.x walks the pieces, blockIdx.y the rows.  Reads gy and the saved tensor, writes dz: HBM-bound.
+// rows at a time; the pieces walk fastest over the workgroups.  Reads gy and the saved tensor, writes dz: HBM-bound.  The weight is transposed by
+// the workgroups behind `act_blocks`, in the same launch.
 // KIND 0: no activation (only the sums), 1: saved is z, 2: saved is y and only its sign matters
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ gy, const void* __restrict__ saved, T* __restrict__ dz,
                                                        float* __restrict__ sums, long P, long C, long ldg, long ld_dz, int lanes, long rows_per_block,
-                                                       int act, float slope) {
+                                                       int act, float slope, int col_blocks, unsigned act_blocks, const T* __restrict__ w,
+                                                       T* __restrict__ wt, int N, int K, int ldt) {
     constexpr int E = Num<T>::E;
-    __shared__ float part[256][E + 1];
-    const int rows = 256 / lanes, r = threadIdx.x / lanes, piece = blockIdx.x * lanes + threadIdx.x % lanes;
-    const long c = (long)piece * E;
-    const long from = blockIdx.y * rows_per_block, to = min(P, from + rows_per_block);
+    __shared__ union {
+        float part[256][E + 1];
+        T tile[64][66];
+    } lds;
+    if (blockIdx.x >= act_blocks) {
+        transpose_weight<T>(lds.tile, w, wt, N, K, ldt, blockIdx.x - act_blocks);
+        return;
+    }
+    auto& part = lds.part;
+    const int rows = 256 / lanes, r = threadIdx.x / lanes, piece = (int)(blockIdx.x % col_blocks) * lanes + threadIdx.x % lanes;
+    const long c = (long)piece * E, row_block = blockIdx.x / col_blocks;
+    const long from = row_block * rows_per_block, to = min(P, from + rows_per_block);
     float acc[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = 0.f;
@@ -832,40 +875,8 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ gy,
         for (int i = 0; i < E && c + i < C; ++i) {
             float t = 0.f;
             for (int q = 0; q < rows; ++q) t += part[q * lanes + threadIdx.x][i];
-            sums[blockIdx.y * C + c + i] = t;
+            sums[row_block * C + c + i] = t;
         }
-    }
-}
-
-// w (groups * N, K) -> wt (groups * K, ldt >= N), columns behind N zero: the data gradient's second operand with n contiguous
-template <typename T>
-__global__ __launch_bounds__(256) void transpose_weight_kernel(const T* __restrict__ w, T* __restrict__ wt, int N, int K, int ldt) {
-    __shared__ T tile[64][66];
-    const int n0 = blockIdx.x * 64, k0 = blockIdx.y * 64;
-    w += (long)blockIdx.z * N * K;
-    wt += (long)blockIdx.z * K * ldt;
-    constexpr int E = Num<T>::E, LPR = 64 / E;
-#pragma unroll
-    for (int j = 0; j < 64 * LPR / 256; ++j) {
-        const int i = j * 256 + threadIdx.x, r = i / LPR, c = i % LPR * E;
-        T v[E];
-        u32x4 piece{0, 0, 0, 0};
-        if (n0 + r < N && k0 + c < K) piece = load_piece(w + (long)(n0 + r) * K, k0 + c, K);
-        __builtin_memcpy(v, &piece, 16);
-#pragma unroll
-        for (int q = 0; q < E; ++q) tile[r][c + q] = v[q];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 64 * LPR / 256; ++j) {
-        const int i = j * 256 + threadIdx.x, r = i / LPR, c = i % LPR * E;
-        if (k0 + r >= K || n0 + c >= ldt) continue;             // ldt is a whole number of pieces
-        T v[E];
-        u32x4 piece;
-#pragma unroll
-        for (int q = 0; q < E; ++q) v[q] = tile[c + q][r];
-        __builtin_memcpy(&piece, v, 16);
-        store16(wt + (long)(k0 + r) * ldt + n0 + c, piece);
     }
 }
 
@@ -1353,11 +1364,12 @@ int launch_bwd(const T* gy, const T* x, const T* w, const void* saved, int kind,
     T* wt = reinterpret_cast<T*>(ws + b.dz);
     float* sums = gb ? reinterpret_cast<float*>(ws + b.dz + b.wt) : nullptr;
     float* split = reinterpret_cast<float*>(ws + b.dz + b.wt + b.sums);
-    if (dz || sums) {
-        const dim3 grid((unsigned)b.col_blocks, (unsigned)b.row_blocks);
+    const unsigned act_blocks = dz || sums ? (unsigned)b.col_blocks * b.row_blocks : 0;
+    const unsigned wt_blocks = gx ? (unsigned)cdiv(b.ldt, 64) * cdiv(K, 64) * groups : 0;
+    if (act_blocks + wt_blocks) {
         auto* kernel = kind == 0 ? &act_grad_kernel<T, 0> : (kind == 1 ? &act_grad_kernel<T, 1> : &act_grad_kernel<T, 2>);
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, gy, saved, dz, sums, (long)P, (long)C, (long)ldg, (long)b.ld_dz, b.lanes,
-                           (long)b.rows_per_block, act, slope);
+        hipLaunchKernelGGL(kernel, dim3(act_blocks + wt_blocks), dim3(256), 0, s, gy, saved, dz, sums, (long)P, (long)C, (long)ldg, (long)b.ld_dz,
+                           b.lanes, (long)b.rows_per_block, act, slope, b.col_blocks, act_blocks, w, wt, N, K, b.ldt);
     }
     const bool padded = dz != nullptr;
     if (padded) {
@@ -1366,7 +1378,6 @@ int launch_bwd(const T* gy, const T* x, const T* w, const void* saved, int kind,
     }
     if (gx) {
         const Epilogue none{};
-        hipLaunchKernelGGL(transpose_weight_kernel<T>, dim3(cdiv(b.ldt, 64), cdiv(K, 64), groups), dim3(256), 0, s, w, wt, N, K, b.ldt);
         // the zeros behind N in dz and in wt's rows are multiplied along: whole pieces
         rows_gemm<T>(gy, wt, gx, P, K, padded && groups == 1 ? b.ldt : N, groups, ldg, b.ldt, (long)groups * K, (long)K * b.ldt, none, s);
     }
