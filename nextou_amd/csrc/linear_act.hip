@@ -1223,7 +1223,7 @@ size_t elem_bytes(int dtype) { return dtype == 0 ? 4 : 2; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // The panel kernel from 65536 rows on: then each of its 2048 waves has 32 rows.  Panel against tiles, us: 65536 rows bfloat16 132 -> 132 15.5 / 27.8,
-// 264 -> 528 48 / 69; 172032 rows 132 -> 528 91 / 164, float32 252 / 467; fewer rows leave waves idle, 21504 rows 132 -> 264 17.4 / 16.0, float32
+// 264 -> 528 48 / 69; 172032 rows 132 -> 528 91 / 164, float32 249 / 330; fewer rows leave waves idle, 21504 rows 132 -> 264 17.4 / 16.0, float32
 // 132 -> 132 34 / 20.  Rows of more than 17 k steps leave no registers for the next rows: 172032 rows 384 -> 384 132 / 117, 400 -> 1600 593 / 484.
 constexpr long kPanelRows = 65536;
 // k split over the waves where fewer than 64 tiles of 64 x 64 would be there, and up to 160 with rows of 4 KB and more.  Split against tiles, us:
