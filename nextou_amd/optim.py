@@ -123,6 +123,8 @@ def _norm_rows(tensors: List[torch.Tensor], in_place: bool):
         if not _flat_run(t):
             if in_place and any(a < b for a, b in _strides_and_reach(t)):
                 raise ValueError("gradient norm: a gradient of shape %s and strides %s overlaps itself" % (tuple(t.shape), t.stride()))
+            if in_place and any(t.data_ptr() == c.data_ptr() for c, _ in copies):
+                raise RuntimeError("gradient norm: two of the gradients share memory (the same one listed twice?)")
             copies.append((t, t.contiguous()))
             t = copies[-1][1]
         vals.extend((t.data_ptr(), n, code))

@@ -207,6 +207,15 @@ class _StandInLib:
         return 0
 
 
+def test_a_strided_gradient_listed_twice_is_refused():
+    base = torch.randn(6, 8)
+    left, right = base[:, :4], base[:, 4:]
+    assert len(optim._norm_rows([left, right, torch.randn(3)], True)[1]) == 2          # interleaved, nothing shared
+    with pytest.raises(RuntimeError, match="share memory"):
+        optim._norm_rows([left, right, left], True)
+    assert len(optim._norm_rows([left, right, left], False)[1]) == 3                    # a norm only reads
+
+
 def test_clip_sgd_clips_over_several_groups(monkeypatch):
     fake = _StandInLib()
     monkeypatch.setattr(_lib, "lib", lambda: fake)
