@@ -24,6 +24,8 @@ infrastructure has installed a checker with :func:`install_cpu_checker` (tests/ 
 from __future__ import annotations
 
 import contextlib
+import ctypes
+import functools
 import math
 import threading
 from typing import Callable, List, Optional
@@ -66,6 +68,11 @@ def _backend_for(t: torch.Tensor):
 
 def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def _raw_stream(index: int) -> int:
+    """:func:`_stream_ptr` without the stream object, for calls whose kernels take a few microseconds."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _f32c(t: torch.Tensor) -> torch.Tensor:
@@ -905,13 +912,13 @@ class _HipBackend:
         """x (P, groups*K) rows with dense columns, w (groups*N, K) dense -> (y (P, groups*N) dense, z for the backward | None)."""
         P, (C, K), dev = x.shape[0], w.shape, x.device
         with _current_device(dev):
-            y = torch.empty((P, C), dtype=x.dtype, device=dev)
-            pre = torch.empty((P, C), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=dev) if want_pre else None
+            y = x.new_empty((P, C))
+            pre = x.new_empty((P, C), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16) if want_pre else None
             rc = _lib.lib().nextou_linear_act_fwd(
                 x.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
                 y.data_ptr(), None if pre is None else pre.data_ptr(), P, C // groups, K, groups, x.stride(0),
                 0 if residual is None else residual.stride(0), C, _LINEAR_TYPES[x.dtype], bias is not None and bias.dtype == torch.float32,
-                act, slope, _stream_ptr(dev))
+                act, slope, _raw_stream(dev.index))
         if rc:
             _lib.check(rc, "linear_act_fwd")
         return y, pre
@@ -919,23 +926,29 @@ class _HipBackend:
     @staticmethod
     def linear_act_bwd(gy, x, w, saved, saved_kind, act, slope, groups, want_gx, want_gw, gb_dtype):
         """(gx (P, groups*K), gw like w, gb (groups*N,)), each None when not wanted; gb_dtype None: no bias gradient."""
-        import ctypes
-        L_ = _lib.lib()
-        P, (C, K) = x.shape[0], w.shape
+        P, (C, K), dev = x.shape[0], w.shape, x.device
         N, code = C // groups, _LINEAR_TYPES[x.dtype]
-        need = ctypes.c_size_t(0)
-        with _current_device(x.device):
-            _lib.check(L_.nextou_linear_act_bwd_workspace(P, N, K, groups, code, act, int(want_gx), int(want_gw), int(gb_dtype is not None),
-                                                          ctypes.byref(need)), "linear_act_bwd_workspace")
-            ws = torch.empty((need.value,), dtype=torch.uint8, device=x.device) if need.value else None
-            gx = torch.empty((P, groups * K), dtype=x.dtype, device=x.device) if want_gx else None
-            gw = torch.empty((C, K), dtype=x.dtype, device=x.device) if want_gw else None
-            gb = torch.empty((C,), dtype=gb_dtype, device=x.device) if gb_dtype is not None else None
-            rc = L_.nextou_linear_act_bwd(gy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(saved), saved_kind, _ptr(gx), _ptr(gw), _ptr(gb),
-                                          _ptr(ws), need.value, P, N, K, groups, gy.stride(0), x.stride(0), code,
-                                          int(gb_dtype == torch.float32), act, slope, _stream_ptr(x.device))
-        _lib.check(rc, "linear_act_bwd")
+        need = _linear_act_bwd_bytes(P, N, K, groups, code, act, want_gx, want_gw, gb_dtype is not None)
+        with _current_device(dev):
+            ws = x.new_empty((need,), dtype=torch.uint8) if need else None
+            gx = x.new_empty((P, groups * K)) if want_gx else None
+            gw = x.new_empty((C, K)) if want_gw else None
+            gb = x.new_empty((C,), dtype=gb_dtype) if gb_dtype is not None else None
+            rc = _lib.lib().nextou_linear_act_bwd(
+                gy.data_ptr(), x.data_ptr(), w.data_ptr(), _ptr(saved), saved_kind, _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), need, P, N, K, groups,
+                gy.stride(0), x.stride(0), code, gb_dtype == torch.float32, act, slope, _raw_stream(dev.index))
+        if rc:
+            _lib.check(rc, "linear_act_bwd")
         return gx, gw, gb
+
+
+@functools.lru_cache(maxsize=256)
+def _linear_act_bwd_bytes(P, N, K, groups, code, act, want_gx, want_gw, want_gb) -> int:
+    """Workspace of a backward call: a plan of the sizes alone."""
+    need = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().nextou_linear_act_bwd_workspace(P, N, K, groups, code, act, want_gx, want_gw, want_gb, ctypes.byref(need)),
+               "linear_act_bwd_workspace")
+    return need.value
 
 
 def _logit_strides(logits, nl, V):
@@ -1808,7 +1821,8 @@ class _LinearAct(torch.autograd.Function):
         sign = act == 1 or (act == 2 and slope >= 0.0)
         kind = 0 if act == 0 else (2 if sign and residual is None and x.dtype != torch.float16 else 1)
         y, pre = be.linear_act_fwd(x2, w2, bias, None if residual is None else _as_rows(residual), act, slope, groups, kind == 1)
-        y = y.view(x.shape[:-1] + (w2.shape[0],))
+        if x.dim() != 2:
+            y = y.view(x.shape[:-1] + (w2.shape[0],))
         ctx.save_for_backward(x, weight, pre if kind == 1 else (y if kind == 2 else None))
         ctx.conf = (kind, act, slope, groups, None if bias is None else bias.dtype)
         return y
@@ -1825,10 +1839,9 @@ class _LinearAct(torch.autograd.Function):
             gb = None if bias_dtype is None else torch.zeros(weight.shape[0], dtype=bias_dtype, device=x.device)
         elif want_x or want_w or want_b:
             gx, gw, gb = _backend_for(x).linear_act_bwd(
-                _as_rows(gy), _as_rows(x), weight.contiguous(), None if saved is None else saved.reshape(-1, weight.shape[0]), kind, act,
-                slope, groups, want_x, want_w, bias_dtype if want_b else None)
-        return (None if gx is None else gx.view(x.shape), None if gw is None else gw.view(weight.shape), gb,
-                gy if ctx.needs_input_grad[3] else None, None, None, None)
+                _as_rows(gy), _as_rows(x), weight.contiguous(), saved if saved is None or saved.dim() == 2 else saved.reshape(-1, weight.shape[0]),
+                kind, act, slope, groups, want_x, want_w, bias_dtype if want_b else None)
+        return (gx if gx is None or x.dim() == 2 else gx.view(x.shape), gw, gb, gy if ctx.needs_input_grad[3] else None, None, None, None)
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
