@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
 import math
 import operator
 import os
@@ -29,6 +30,7 @@ from typing import Iterable, List, Optional, Union
 import torch
 
 from . import _lib
+from .graph_ops import _current_device, _raw_stream
 
 __all__ = ["ClipSGD", "clip_grad_norm_", "grad_norm"]
 
@@ -139,21 +141,28 @@ def _strides_and_reach(t: torch.Tensor):
         reach += stride * (n - 1)
 
 
+@functools.lru_cache(maxsize=64)
+def _multi_norm_bytes(n: int) -> int:
+    need = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().nextou_multi_norm_workspace(n, ctypes.byref(need)), "multi_norm_workspace")
+    return need.value
+
+
 def _multi_norm(tensors: List[torch.Tensor], code: int, max_norm: float, scale: bool) -> torch.Tensor:
     """float32 (norm, clip factor) of device tensors; ``scale`` multiplies them by the factor in place."""
-    device = tensors[0].device
-    with _on_device(device):
+    first = tensors[0]
+    device = first.device
+    with _current_device(device):
         vals, copies = _norm_rows(tensors, scale)
         if not vals:
             return torch.zeros(2, device=device)          # only empty tensors
         n, L = len(vals) // 3, _lib.lib()
-        need = ctypes.c_size_t(0)
-        _lib.check(L.nextou_multi_norm_workspace(n, ctypes.byref(need)), "multi_norm_workspace")
-        ws = torch.empty((need.value,), dtype=torch.uint8, device=device)
-        out = torch.empty((2,), dtype=torch.float32, device=device)
+        need = _multi_norm_bytes(n)
+        ws, out = first.new_empty((need,), dtype=torch.uint8), first.new_empty((2,), dtype=torch.float32)
         call = L.nextou_multi_clip if scale else L.nextou_multi_norm
-        _lib.check(call(vals.buffer_info()[0], n, code, max_norm, ws.data_ptr(), need.value, out.data_ptr(), _stream_of(device)),
-                   "multi_clip" if scale else "multi_norm")
+        rc = call(vals.buffer_info()[0], n, code, max_norm, ws.data_ptr(), need, out.data_ptr(), _raw_stream(device.index))
+        if rc:
+            _lib.check(rc, "multi_clip" if scale else "multi_norm")
         if scale:
             for t, dense in copies:
                 t.copy_(dense)
