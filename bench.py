@@ -92,7 +92,7 @@ def move_to(trainer, device, fused_sgd=False):
     # fused_sgd: torch's single-launch multi-tensor SGD (same update rule; -0.5 ms per cfg-2 step).  Only without the gradient averager:
     # the averaged step's gradients are views into the flat buckets and keeps the foreach implementation.  (The GPU memory fault round 4
     # first blamed on this combination is MIOpen's backward-data kernel of the 1x1 head convolution reading past its operand —
-    # tools/conv_bwd_fault_repro.py, profiles/r05_n_gt_1.md; the heads run on K8 since.)
+    # profiles/r05_n_gt_1.md; the heads run on K8 since.)
     fused = fused_sgd and device.type == "cuda" and os.environ.get("NEXTOU_SGD_FUSED", "1") != "0"
     if device.type == "cuda" and os.environ.get("NEXTOU_CLIP_SGD", "1") != "0":
         # round 5: the clip and the update on the library's step-glue kernels (nextou_amd/optim.py: a torch.optim.SGD whose step names

@@ -4,7 +4,7 @@
 // Reference: the deep-supervision `seg_layers` of the decoder (NexToU_Encoder_Decoder.py:253-258 build, :311-337 forward:
 // `self.seg_layers[s](x)` — nn.Conv3d(features, num_classes, 1, 1, 0, bias=True)).  PyTorch-ROCm hands them to MIOpen as
 // convolutions; the backward of the full-resolution head is the call the averaged (N > 1) eager step died in with a GPU
-// memory fault (profiles/r04_sgd_fused.md, tools/conv_bwd_fault_repro.py), so the heads moved onto kernels of this library.
+// memory fault (profiles/r05_n_gt_1.md), so the heads moved onto kernels of this library.
 //
 // The problem is HBM-bound by a wide margin (cfg 2, full resolution: 5.5 M points x (40 -> 14): 216 B and 1 120 flop per
 // point), L <= 16 per tile is far below any GEMM tile, and the rows (160 B and 56 B) are shorter than a wave's access, so

@@ -1,8 +1,7 @@
 """The N > 1 path on the one GPU of a test box: the bucketed, overlapped gradient mean of
 nextou_amd/ddp.py over RCCL (`nccl`, world size 1) — eager and captured into a hipGraph — against the plain step; bench.py's
 averaged step end to end; two ranks sharing the GPU over gloo.  No retries, no skips: the GPU memory fault these paths used to hit
-was MIOpen's backward-data kernel of the 1x1 head convolution reading past its operand (tools/conv_bwd_fault_repro.py,
-profiles/r05_n_gt_1.md), and the heads now run on K8 (csrc/head_rows.hip)."""
+was MIOpen's backward-data kernel of the 1x1 head convolution reading past its operand (profiles/r05_n_gt_1.md), and the heads now run on K8 (csrc/head_rows.hip)."""
 import json
 import os
 import subprocess

@@ -3,8 +3,8 @@
 Every input, every output and every workspace of a launch lives in a guard-page buffer (tools/guard_alloc.py: HIP virtual-memory
 API, the pages before and after the mapping are unmapped).  First pass: every buffer ENDS on the guard (a read or write past the last
 element faults); second pass: every buffer STARTS on the guard (a negative offset faults).  A fault is `Memory access fault by GPU`
-and kills the process — the test then fails as a crashed run, exactly like the library convolution of
-tools/conv_bwd_fault_repro.py did under the N > 1 step (profiles/r05_n_gt_1.md).  The results of the guarded launches are
+and kills the process — the test then fails as a crashed run, exactly like a library convolution
+did under the N > 1 step (profiles/r05_n_gt_1.md).  The results of the guarded launches are
 compared with the same launch on caching-allocator tensors: bit-identical for the kernels with a fixed summation order, to
 round-off for those that accumulate with float atomics.
 

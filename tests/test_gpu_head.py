@@ -2,7 +2,7 @@
 stage's features to the class logits (reference NexToU_Encoder_Decoder.py:253-258, :311-337) and their autograd, against the
 float64 convolution of the same operands; bit-reproducibility; operands in guard-page buffers (tools/guard_alloc.py: the byte
 after an operand's last element is unmapped — the library convolution this replaces fails exactly that test,
-tools/conv_bwd_fault_repro.py); the model takes the kernels at every head."""
+profiles/r05_n_gt_1.md); the model takes the kernels at every head."""
 import pytest
 import torch
 import torch.nn.functional as F

@@ -3,8 +3,7 @@
 HIP's virtual-memory API (hipMemAddressReserve / hipMemCreate / hipMemMap / hipMemSetAccess) lets a test place a buffer
 so that the byte after its last element (and the byte before its first) belongs to no mapping: a kernel that reads or writes
 past an operand takes a `Memory access fault by GPU` deterministically, instead of only when the caching allocator happens
-to have left the neighbouring page unmapped.  Used by tools/conv_bwd_fault_repro.py (the N > 1 step's fault
-item 1a) and by tests/test_gpu_guard.py (no kernel of libnextou_hip.so reads past its operands).
+to have left the neighbouring page unmapped.  Used by tests/test_gpu_guard.py (no kernel of libnextou_hip.so reads past its operands).
 
 Test / tool infrastructure only: nothing under nextou_amd/ imports this.
 """

@@ -12,13 +12,8 @@
 #   pmcmrg     the same two PMC passes over the K2 + K7 kernel and the three launches it replaces (tools/kernel_bench.py --mrg)
 #   pmcjson    regenerate profiles/pmc_traffic.json (-> <out>/pmc_traffic.json) for the labels that launch today
 #   convtable  per-layer table of the library convolutions at the model's own routing (tools/conv_layer_table.py)
-#   heads      K8 against the library route at the cfg-2 head shapes
-#   repro      the guard-page reproducer of MIOpen's backward-data over-read (+ K8 on the same operands)
-#   reprobf16  the guard-page reproducer with bf16 operands (tiny and cfg-2 head shapes) + two bf16 bench lines: the reduced-precision fault
-#              of round 5's closing tree
-#   bf16       round 6: bench.py --autocast-bf16 at cfg 2 / tiny / cfg 5 in find mode, twice each; on a fault a serialized rerun with MIOpen's log
-#   bf16ab     round 6: round 5's faulting bf16 configuration (NEXTOU_REDUCED_PRECISION_FILTERS=stored) three times; on a fault once more with synchronous
-#              launches and MIOpen's command log (profiles/r06_bf16/README.md)
+#   heads      K8 at the cfg-2 head shapes
+#   bf16       bench.py --autocast-bf16 at cfg 2 / tiny / cfg 5 in find mode, twice each; ends at the first run that fails
 #   stem       round 6: K9 / DDP tests + the headline line with and without the stem block on one box
 #   k1small    round 6: small-graph kNN tests, tools/stem_bench.py, the K1 rows of the kernel bench with and without knn_small_kernel
 #   ab6        round 6: same-box A/B of the step changes (K9, small kNN, skip fork) against the round-5 routing (profiles/r06_step_ab.md)
@@ -29,14 +24,11 @@
 #   pwmodes    stage 3-5 blocks with the point-wise convolutions on the library route / on K7 / K7 weight gradient only, replayed graphs
 #   stepglue   tests of the step-glue kernels (ClipSGD, narrow_copy_sum) + tools/step_ab.py: the bench step against variants without
 #              clip / optimizer and with the own clip + SGD kernels, captured side by side and replayed in alternation
-#   optim      tools/optim_bench.py (clip + SGD alone: torch's multi-tensor kernels against ClipSGD) + the RCCL capture / watchdog
-#              reproducer (tools/rccl_capture_watchdog_repro.py) + the averaged-step test
+#   optim      tools/optim_bench.py (clip + SGD alone: torch's multi-tensor kernels against ClipSGD) + the averaged-step test
 #   sgdab      bench.py in separate processes, alternating: default (ClipSGD) against NEXTOU_CLIP_SGD=0 (torch's fused SGD + clip) — the
 #              process-level A/B of the optimizer inside the replayed step — and the averaged-step test four times over
 #   benchfinal the headline line (default: ClipSGD, one-pass concatenation backward, up-convolutions as GEMMs; with cpu_baseline) and the same
 #              step with NEXTOU_CLIP_SGD=0 (torch's clip + fused SGD)
-#   averaged   bench.py --force-averager --graph on at cfg 2: the N > 1 step (hooks, buckets, RCCL collectives on a world-size-1 group) at the
-#              closing tree, next to the plain step's line
 #   cpusurvey  bench.py --cpu-protocol survey (batch 2, 1 + 3 steps, all physical cores; ~10 min of host time)
 #   closing    tests margins bench configs stages kernels trace pmc5 pmcmrg in that order
 TASK=${1:-closing}
@@ -89,7 +81,6 @@ t_stepglue() {
   python tools/step_ab.py --rounds 3 --steps 10 --eager > $OUT/step_ab.txt 2> $OUT/step_ab.log; tail -8 $OUT/step_ab.txt; tail -3 $OUT/step_ab.log
 }
 t_optim() {
-  python tools/rccl_capture_watchdog_repro.py 3 > $OUT/rccl_capture_watchdog_repro.txt 2>&1; cat $OUT/rccl_capture_watchdog_repro.txt
   python tools/optim_bench.py 2>&1 | grep -v "amdgpu.ids" > $OUT/optim_bench.txt; cat $OUT/optim_bench.txt
   python -m pytest tests/test_gpu_ddp.py -q -m gpu -rf -k "averaged_step" 2>&1 | grep -v "MIOpen\|amdgpu.ids" | tail -5 > $OUT/ddp_pytest.txt; tail -3 $OUT/ddp_pytest.txt
 }
@@ -106,10 +97,6 @@ t_benchfinal() {
   python bench.py > $OUT/bench_cfg2_default.json 2> $OUT/bench_cfg2_default.log; field $OUT/bench_cfg2_default.json
   python -c "import json;d=json.load(open('$OUT/bench_cfg2_default.json'));print(d['config']['optimizer']);print({k:(v['avg_us'],v['frac']) for k,v in d['roofline_graph'].items() if v and k.startswith('glue')})"
   NEXTOU_CLIP_SGD=0 python bench.py --no-cpu-baseline > $OUT/bench_cfg2_torch_sgd.json 2>/dev/null; field $OUT/bench_cfg2_torch_sgd.json
-}
-t_averaged() {
-  python bench.py --no-cpu-baseline --steps 10 --warmup 3 --force-averager --graph on > $OUT/bench_cfg2_averaged.json 2> $OUT/bench_cfg2_averaged.log; field $OUT/bench_cfg2_averaged.json
-  python -c "import json;d=json.load(open('$OUT/bench_cfg2_averaged.json'));print(d['config']['optimizer'], d['dist']['backend'], d['config']['gradient_averager'])"
 }
 t_trace() {
   cd /tmp && export TMPDIR=/tmp
@@ -171,40 +158,16 @@ t_convtable() {
   python tools/conv_layer_table.py --iters 5 --md $OUT/conv_layer_table.md > $OUT/conv_layer_table.log 2>&1; tail -3 $OUT/conv_layer_table.md | cut -c1-300
 }
 t_heads() {
-  python tools/head_bench.py 2>&1 | grep -v "GridwiseOp\|amdgpu.ids\|MIOpen" > $OUT/head_bench.txt; tail -1 $OUT/head_bench.txt
+  python tools/head_bench.py --own-only 2>&1 | grep -v "GridwiseOp\|amdgpu.ids\|MIOpen" > $OUT/head_bench.txt; tail -1 $OUT/head_bench.txt
 }
-t_repro() {
-  python tools/conv_bwd_fault_repro.py --own --repeat 3 --log-dir $OUT/repro_logs 2>&1 | cut -c1-420 > $OUT/conv_bwd_fault_repro.txt; tail -20 $OUT/conv_bwd_fault_repro.txt | cut -c1-160
-}
-t_reprobf16() {      # next round's first call: the bf16 head convolution on guard pages + the reduced-precision bench lines (known issue)
-  python tools/conv_bwd_fault_repro.py --dtype bf16 --repeat 3 --log-dir $OUT/repro_bf16_logs 2>&1 | cut -c1-420 > $OUT/conv_bwd_fault_repro_bf16.txt; tail -20 $OUT/conv_bwd_fault_repro_bf16.txt | cut -c1-160
-  python tools/conv_bwd_fault_repro.py --dtype bf16 --size cfg2 --repeat 2 --log-dir $OUT/repro_bf16_logs 2>&1 | cut -c1-420 > $OUT/conv_bwd_fault_repro_bf16_cfg2.txt; tail -20 $OUT/conv_bwd_fault_repro_bf16_cfg2.txt | cut -c1-160
-  for i in 1 2; do python bench.py --no-cpu-baseline --steps 10 --warmup 3 --autocast-bf16 > $OUT/bench_cfg2_bf16_$i.json 2> $OUT/bench_cfg2_bf16_$i.log; field $OUT/bench_cfg2_bf16_$i.json || tail -2 $OUT/bench_cfg2_bf16_$i.log; done
-}
-t_bf16() {           # round 6: the reduced-precision bench path at HEAD — does it complete in find mode?  On a fault: the same run once more with
-  # synchronous launches and MIOpen's command log, whose tail names the solver that was running (profiles/r06_bf16_*)
+t_bf16() {           # the reduced-precision bench path in find mode; the first run that does not end well ends the task
   for w in "cfg2 10" "tiny 5" "cfg5 5"; do set -- $w
     for i in 1 2; do
-      timeout 1200 python bench.py --no-cpu-baseline --steps $2 --warmup 3 --workload $1 --autocast-bf16 > $OUT/bench_$1_bf16_$i.json 2> $OUT/bench_$1_bf16_$i.log
-      rc=$?; echo "bench $1 bf16 run $i rc $rc"; grep -h "Memory access fault" $OUT/bench_$1_bf16_$i.log | head -2
-      if [ $rc -eq 0 ]; then field $OUT/bench_$1_bf16_$i.json; else
-        MIOPEN_LOG_LEVEL=6 MIOPEN_ENABLE_LOGGING_CMD=1 HIP_LAUNCH_BLOCKING=1 AMD_SERIALIZE_KERNEL=3 timeout 1500 python bench.py --no-cpu-baseline --steps 2 --warmup 1 --workload $1 --autocast-bf16 2>&1 >/dev/null | grep -v "GridwiseOp\|amdgpu.ids" | tail -c 300000 > $OUT/bench_$1_bf16_${i}_serialized_tail.log
-        echo "serialized rerun rc ${PIPESTATUS[0]}"; grep -E "Memory access fault|MIOpenDriver|Solver|solver_id|SolverName" $OUT/bench_$1_bf16_${i}_serialized_tail.log | tail -8 | cut -c1-300
-        break
-      fi
+      timeout -k 10 1200 python bench.py --no-cpu-baseline --steps $2 --warmup 3 --workload $1 --autocast-bf16 > $OUT/bench_$1_bf16_$i.json 2> $OUT/bench_$1_bf16_$i.log
+      rc=$?; echo "bench $1 bf16 run $i rc $rc"
+      if [ $rc -ne 0 ]; then tail -3 $OUT/bench_$1_bf16_$i.log; exit $rc; fi
+      field $OUT/bench_$1_bf16_$i.json
     done
-  done
-}
-t_bf16ab() {         # round 6: the configuration of round 5's faulting bf16 run (channels-last stored filters reach the library under autocast), 3 runs,
-  # then the same with synchronous launches + MIOpen's log if one of them faults: convicts or clears the filter layout
-  for i in 1 2 3; do
-    NEXTOU_REDUCED_PRECISION_FILTERS=stored timeout 900 python bench.py --no-cpu-baseline --steps 5 --warmup 3 --autocast-bf16 > $OUT/bench_cfg2_bf16_stored_$i.json 2> $OUT/bench_cfg2_bf16_stored_$i.log
-    rc=$?; echo "bf16 stored-filter run $i rc $rc"; grep -h "Memory access fault" $OUT/bench_cfg2_bf16_stored_$i.log | head -2
-    if [ $rc -ne 0 ]; then
-      NEXTOU_REDUCED_PRECISION_FILTERS=stored MIOPEN_LOG_LEVEL=6 MIOPEN_ENABLE_LOGGING_CMD=1 HIP_LAUNCH_BLOCKING=1 AMD_SERIALIZE_KERNEL=3 timeout 1500 python bench.py --no-cpu-baseline --steps 2 --warmup 1 --autocast-bf16 2>&1 >/dev/null | grep -v "GridwiseOp\|amdgpu.ids" | tail -c 300000 > $OUT/bench_cfg2_bf16_stored_serialized_tail.log
-      echo "serialized rerun rc ${PIPESTATUS[0]}"; grep -E "Memory access fault|MIOpenDriver|Solver|solver_id|SolverName" $OUT/bench_cfg2_bf16_stored_serialized_tail.log | tail -8 | cut -c1-300
-      break
-    else field $OUT/bench_cfg2_bf16_stored_$i.json; fi
   done
 }
 t_stem() {           # round 6: K9 tests + the headline line with and without the stem block on the same box
@@ -274,7 +237,7 @@ t_cpusurvey() {
   python -c "import json;d=json.load(open('$OUT/bench_cfg2_cpu_survey.json'));print(d['cpu_baseline'])"
 }
 case $TASK in
-  closing) for t in tests margins bench configs stages kernels heads trace convtable pmcjson repro; do echo "== $t"; t_$t; done ;;
+  closing) for t in tests margins bench configs stages kernels heads trace convtable pmcjson; do echo "== $t"; t_$t; done ;;
   *) for t in ${TASK//,/ }; do echo "== $t"; t_$t; done ;;
 esac
 du -sh $OUT | tail -1
