@@ -159,15 +159,11 @@ def filter_layout_for(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     stored layout saves on the default, all-channels-last path.  A channels-last input — dense NDHWC, or the single-channel image
     re-strided by layout.to_channels_last — has stride 1 on its channel axis.
 
-    Reduced precision (bf16 / fp16 autocast) always gets the contiguous form: autocast's cast keeps a filter's strides, and the library's
-    reduced-precision solvers for channels-last FILTERS were never part of a clean measured run — the one `bench.py --autocast-bf16` run of
-    the tree that stored filters channels-last ended in a GPU memory fault (known issue), while contiguous filters are
-    what every earlier bf16 / fp16 run and test used."""
+    Reduced precision (bf16 / fp16 autocast) always gets the contiguous form: autocast's cast keeps a filter's strides, and a library
+    backward-data solver that its find pass tries on channels-last 16-bit filters has ended a training step in a GPU memory fault."""
     if w.dim() < 4 or not x.is_cuda or w.is_contiguous() or x.dim() != w.dim():
         return w
-    if x.stride(1) == 1 and (runs_in_fp32(x) or os.environ.get("NEXTOU_REDUCED_PRECISION_FILTERS", "contiguous") == "stored"):
-        # ("stored": the channels-last filter under autocast too — the configuration of round 5's faulting run, kept reachable for the
-        # A/B that convicts or clears it, profiles/r06_bf16/)
+    if x.stride(1) == 1 and runs_in_fp32(x):
         return w
     return w.contiguous()
 
