@@ -10,7 +10,7 @@ Workload (SURVEY.md §8d cfg 2): 3-D NexToU, patch 64x
 max 324 features, 6 stages, 14 classes, batch 2 per GPU, fp32, BatchNorm in train mode,
 deep-supervision-weighted cross-entropy; synthetic N(0,1) volumes and random-init (He) weights.
 One step = zero_grad -> forward (5 heads) -> loss -> backward -> (N > 1: bucketed RCCL gradient
-average; default: two hipGraphs around the eager all-reduces, `--graph off | on` overlap them with backward)
+average; default: two hipGraphs around the eager all-reduces, `--graph off` overlaps them with backward)
 -> clip_grad_norm_(12) -> SGD(nesterov).  `value` = all ranks'
 voxels / max-over-ranks time of exactly K steps between barrier + synchronize pairs.
 
@@ -407,12 +407,15 @@ def main():
                     help="how the step is replayed.  auto: N = 1 -> ONE captured hipGraph (harness.GraphedTrainStep; cfg 4: the BTI target "
                          "validation runs on the device, checked after timing); with a process group up (N > 1, --force-averager) -> `split`: two "
                          "hipGraphs around EAGER bucket all-reduces (harness.SplitGraphedTrainStep) — no collective is captured, because capturing "
-                         "RCCL collectives can end in an uncatchable abort inside PyTorch's watchdog thread (DESIGN.md 6).  auto falls back to the "
-                         "eager step if a capture fails (error reported in the JSON line).  on: one graph, collectives included (raises if the "
-                         "capture fails); off: the eager step")
+                         "RCCL collectives can end in an uncatchable abort inside PyTorch's watchdog thread.  auto falls back to the "
+                         "eager step if a capture fails (error reported in the JSON line).  on: one graph (raises if the capture fails); "
+                         "refused with a process group; off: the eager step")
     ap.add_argument("--channels-last", action="store_true",
                     help="experiment: run the dense stages in channels_last_3d (NDHWC) memory format")
     args = ap.parse_args()
+    if args.graph == "on" and (args.gpus > 1 or args.force_averager):
+        ap.error("--graph on would capture the collectives of the averaged step, which can end the process inside PyTorch's watchdog thread: "
+                 "use --graph split (the default with a process group) or off")
 
     # `python bench.py --gpus N` typed without a launcher (the round driver's command shape): start the N ranks here
     if needs_self_launch(args.gpus):
@@ -457,17 +460,16 @@ def main():
 
     for _ in range(args.warmup):
         step()
-    # auto: the whole step as one hipGraph, N = 1 and N > 1 alike (the averaged step is capturable: RCCL collectives on their
-    # own stream, no host synchronisation in the hooks or in finalize() once the warm-up steps have seen the gradient pattern)
+    # auto: the whole step as one hipGraph at N = 1
     # (gloo — the two-ranks-on-one-GPU test backend — synchronises with the host inside its collectives and cannot be captured)
     # round 6: with a process group up the default keeps the collectives OUT of any capture — two graphs
-    # around eager all-reduces; the single graph with captured collectives stays available under `--graph on`
+    # around eager all-reduces
     split = args.graph == "split" or (args.graph == "auto" and averager is not None)
     want_graph = args.graph in ("on", "split") or args.graph == "auto"
-    graph_mode = ("one graph, collectives captured (--graph on)" if args.graph == "on" else "eager (--graph off)" if args.graph == "off" else
+    graph_mode = ("one graph (--graph on)" if args.graph == "on" else "eager (--graph off)" if args.graph == "off" else
                   "one graph (auto: no process group)" if not split else
                   "two graphs around eager collectives (%s)" % ("--graph split" if args.graph == "split" else
-                                                                "auto: a process group is up; RCCL collectives are captured only on --graph on"))
+                                                                "auto: a process group is up"))
     graphed, capture_error = None, None
     if want_graph:
         try:

@@ -68,6 +68,10 @@ def _dense_strides(p: torch.Tensor) -> bool:
     return True
 
 
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class BucketedGradientAverager:
     """Overlapped, bucketed all-reduce (mean) of ``module``'s gradients.
 
@@ -85,6 +89,10 @@ class BucketedGradientAverager:
     one per parameter (362 for cfg 2), 2 x 122.7 MB of traffic = ~50 us at HBM speed against a ~230 ms backward.
     A parameter no rank produced a gradient for (the zero-weighted lowest deep-supervision head) keeps ``p.grad = None``,
     exactly as in a single-process step, so momentum / weight decay treat it the same at every world size.
+
+    A collective is never captured into a hipGraph: a step that would do so raises RuntimeError (``zero_grad``, before anything of it is
+    recorded; the launches themselves as well).  PyTorch's watchdog thread of the process group has ended processes during such captures, about
+    once in 25, for a reason that is not established.  ``defer_collectives`` and harness.SplitGraphedTrainStep replay the step around eager ones.
     """
 
     def __init__(self, module: torch.nn.Module, bucket_bytes: int = 32 << 20,
@@ -143,9 +151,16 @@ class BucketedGradientAverager:
     def zero_grad(self) -> None:
         """``optimizer.zero_grad(set_to_none=True)`` for the averaged parameters: the next backward writes fresh
         gradients (no accumulate-into-zeros pass), the flat buckets stay allocated."""
+        if not self.defer_collectives:
+            self._refuse_capture()
         for b in self.buckets:
             for p in b.params:
                 p.grad = None
+
+    def _refuse_capture(self) -> None:
+        if self.buckets and _capturing(self.buckets[0].flat.device):
+            raise RuntimeError("BucketedGradientAverager: collectives are not captured into a hipGraph (the process group's watchdog thread can "
+                               "end the process); set defer_collectives and replay the step with harness.SplitGraphedTrainStep")
 
     @torch.no_grad()
     def _missing_index(self, b: _Bucket, pattern) -> torch.Tensor:
@@ -167,6 +182,7 @@ class BucketedGradientAverager:
 
     @torch.no_grad()
     def _reduce(self, b: _Bucket) -> None:
+        self._refuse_capture()
         b.work = dist.all_reduce(b.flat, op=dist.ReduceOp.SUM, group=self.group, async_op=True)
 
     @torch.no_grad()

@@ -30,7 +30,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run on the GPU box with -m gpu)")
 
 
+# A step with RCCL collectives inside a captured graph now and then ends the process in PyTorch's watchdog thread; the cause is not known, so the
+# mode raises an error and its tests stay off
+_CAPTURED_COLLECTIVES = "captured RCCL collectives can end the process in PyTorch's watchdog thread (cause not established): the mode is switched off"
+_OFF = {
+    "test_gpu_ddp.py::test_explicitly_captured_rccl_step_matches_plain_step": _CAPTURED_COLLECTIVES,
+    "test_gpu_ddp.py::test_bench_averaged_step_on_one_gpu[on]": _CAPTURED_COLLECTIVES,
+}
+
+
 def pytest_collection_modifyitems(config, items):
+    for item in items:
+        for name, reason in _OFF.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.skip(reason=reason))
     if torch.cuda.is_available():
         return
     skip = pytest.mark.skip(reason="no GPU in this container")
