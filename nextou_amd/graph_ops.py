@@ -31,6 +31,7 @@ import threading
 from typing import Callable, List, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -88,6 +89,15 @@ _NO_CONTEXT = contextlib.nullcontext()
 def _current_device(device: torch.device):
     """``torch.cuda.device(device)``, without its cost where that is the current one."""
     return _NO_CONTEXT if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_tracing_state = torch._C._get_tracing_state
+
+
+def _recorded() -> bool:
+    """Whether torch keeps a record of the operations without any tensor requiring a gradient: forward-mode derivatives, or a trace.  A kernel
+    that fills an empty tensor by its address is not in such a record."""
+    return forward_ad._current_level >= 0 or _tracing_state() is not None
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -1855,7 +1865,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     float32, bfloat16 or float16; all tensors of one type, except that the bias may be float32 beside 16-bit rows.  Sums are held in
     float32 and every output and gradient is rounded once (with an activation in 16 bits, so is d loss / d z on its way into the two
     gradient products).  Under autocast the tensors are cast to the autocast type first.  Any sizes and any strides: columns that are not
-    dense are copied, an expanded row is read as it is.  Gradients are bit-reproducible; there is no double backward.
+    dense are copied, an expanded row is read as it is.  Gradients are bit-reproducible; there is no double backward and no forward-mode
+    derivative (NotImplementedError for a tensor with a tangent).
     ValueError / TypeError for shapes, types or devices that do not fit."""
     if act not in _LINEAR_ACTS:
         raise ValueError("linear_act: act %r is none of %s" % (act, ", ".join(sorted(_LINEAR_ACTS))))
@@ -1883,7 +1894,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     training = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
                                             (residual is not None and residual.requires_grad))
-    if not training and x.numel():
+    if not training and x.numel() and not _recorded():
         y, _ = _backend_for(x).linear_act_fwd(_as_rows(x), weight.contiguous(), bias, None if residual is None else _as_rows(residual),
                                               _LINEAR_ACTS[act], float(negative_slope), groups, False)
         return y if x.dim() == 2 else y.view(x.shape[:-1] + (weight.shape[0],))
