@@ -30,7 +30,7 @@ from typing import Iterable, List, Optional, Union
 import torch
 
 from . import _lib
-from .graph_ops import _current_device, _raw_stream
+from .graph_ops import _current_device, _raw_stream, _recorded
 
 __all__ = ["ClipSGD", "clip_grad_norm_", "grad_norm"]
 
@@ -173,12 +173,13 @@ def _multi_norm(tensors: List[torch.Tensor], code: int, max_norm: float, scale: 
 def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """The ``norm_type``-norm (1, 2 or inf) of all elements of ``tensors`` taken together, as a 0-dim float32 tensor on their device (no host
     synchronisation): what ``torch.nn.utils.get_total_norm`` returns, for float32 / bfloat16 / float16 tensors in one list, with float64 sums
-    in a fixed order.  NaN if any element is.  An empty list gives 0.  TypeError / ValueError for other types and mixed devices."""
+    in a fixed order.  NaN if any element is.  An empty list gives 0.  TypeError / ValueError for other types and mixed devices.  CPU tensors,
+    and what a trace or a forward-mode derivative records, go through torch's implementation."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     code = _norm_code(norm_type)
     if not tensors:
         return torch.tensor(0.0)
-    if not tensors[0].is_cuda:
+    if not tensors[0].is_cuda or _recorded():
         return torch.nn.utils.get_total_norm(tensors, float(norm_type)).float()
     return _multi_norm(tensors, code, math.inf, False)[0]
 
@@ -191,7 +192,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
 
     Gradients may be float32, bfloat16 and float16 in one list, of any dense layout (others are copied and written back).  A norm that is
     infinite or NaN scales as in torch: to zeros and NaN.  No two gradients may share memory (a parameter listed twice: RuntimeError).
-    CPU gradients go through torch's implementation; ``foreach`` is accepted for its signature.  Capturable: the gradients' addresses and
+    CPU gradients, and what a trace or a forward-mode derivative records, go through torch's implementation; ``foreach`` is accepted for its signature.  Capturable: the gradients' addresses and
     ``max_norm`` are those of the capture."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     code, max_norm = _norm_code(norm_type), float(max_norm)
@@ -200,7 +201,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     grads = [g for g in map(_GRAD, parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    if not grads[0].is_cuda:
+    if not grads[0].is_cuda or _recorded():
         return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite, foreach)
     if error_if_nonfinite:
         norm = _multi_norm(grads, code, max_norm, False)[0]
