@@ -88,6 +88,18 @@ _DTYPE, _DEVICE = operator.attrgetter("dtype"), operator.attrgetter("device")
 _GRAD = operator.attrgetter("grad")
 
 
+class _NotTaken(Exception):
+    """Tensors that the kernels do not take and torch's implementation may."""
+
+
+class _OtherTypes(_NotTaken, TypeError):
+    pass
+
+
+class _OtherDevices(_NotTaken, ValueError):
+    pass
+
+
 def _norm_code(norm_type) -> int:
     code = _NORM_CODES.get(float(norm_type))
     if code is None:
@@ -106,22 +118,25 @@ def _norm_rows(tensors: List[torch.Tensor], in_place: bool):
         if all(map(torch.Tensor.is_contiguous, tensors)):
             counts, types = list(map(torch.Tensor.numel, tensors)), list(map(_NORM_TYPES.get, map(_DTYPE, tensors)))
             if None not in types and 0 not in counts and len(set(map(_DEVICE, tensors))) == 1:
-                vals = array.array("q", bytes(24 * len(tensors)))
-                vals[0::3] = array.array("q", map(torch.Tensor.data_ptr, tensors))      # (a tensor without storage raises here)
-                vals[1::3], vals[2::3] = array.array("q", counts), array.array("q", types)
-                return vals, []
+                at = array.array("q", map(torch.Tensor.data_ptr, tensors))              # (a tensor without storage raises here, or has address 0)
+                if 0 not in at:
+                    vals = array.array("q", bytes(24 * len(tensors)))
+                    vals[0::3], vals[1::3], vals[2::3] = at, array.array("q", counts), array.array("q", types)
+                    return vals, []
     except (RuntimeError, NotImplementedError):
         pass
     device, vals, copies = tensors[0].device, array.array("q"), []
     for t in tensors:
         code = _NORM_TYPES.get(t.dtype)
         if code is None or t.layout is not torch.strided:
-            raise TypeError("gradient norm: dense float32, bfloat16 or float16 gradients, got %s %s" % (t.layout, t.dtype))
+            raise _OtherTypes("gradient norm: dense float32, bfloat16 or float16 gradients, got %s %s" % (t.layout, t.dtype))
         if t.device != device:
-            raise ValueError("gradient norm: gradients on %s and %s" % (device, t.device))
+            raise _OtherDevices("gradient norm: gradients on %s and %s" % (device, t.device))
         n = t.numel()
         if n == 0:
             continue
+        if not t.data_ptr():
+            raise _OtherTypes("gradient norm: a %s without memory of its own" % type(t).__name__)
         if not _flat_run(t):
             if in_place and any(a < b for a, b in _strides_and_reach(t)):
                 raise ValueError("gradient norm: a gradient of shape %s and strides %s overlaps itself" % (tuple(t.shape), t.stride()))
@@ -192,7 +207,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
 
     Gradients may be float32, bfloat16 and float16 in one list, of any dense layout (others are copied and written back).  A norm that is
     infinite or NaN scales as in torch: to zeros and NaN.  No two gradients may share memory (a parameter listed twice: RuntimeError).
-    CPU gradients, and what a trace or a forward-mode derivative records, go through torch's implementation; ``foreach`` is accepted for its signature.  Capturable: the gradients' addresses and
+    What the kernels do not take — CPU gradients, other types, sparse and distributed ones, several devices, a trace, a forward-mode derivative — goes
+    through torch's implementation, for the same three norms; ``foreach`` is accepted for its signature.  Capturable: the gradients' addresses and
     ``max_norm`` are those of the capture."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     code, max_norm = _norm_code(norm_type), float(max_norm)
@@ -201,13 +217,16 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     grads = [g for g in map(_GRAD, parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    if not grads[0].is_cuda or _recorded():
-        return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite, foreach)
-    if error_if_nonfinite:
-        norm = _multi_norm(grads, code, max_norm, False)[0]
-        if not math.isfinite(norm.item()):
-            raise RuntimeError("The total norm of order %s for gradients from `parameters` is non-finite, so it cannot be clipped." % norm_type)
-    return _multi_norm(grads, code, max_norm, True)[0]
+    if grads[0].is_cuda and not _recorded():
+        try:
+            if error_if_nonfinite:
+                norm = _multi_norm(grads, code, max_norm, False)[0]
+                if not math.isfinite(norm.item()):
+                    raise RuntimeError("The total norm of order %s for gradients from `parameters` is non-finite, so it cannot be clipped." % norm_type)
+            return _multi_norm(grads, code, max_norm, True)[0]
+        except _NotTaken:                     # (raised before anything is launched)
+            pass
+    return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite, foreach)
 
 
 class _Table:

@@ -100,3 +100,66 @@ def test_a_tangent_is_not_dropped(kernels):
                 continue
             assert fwAD.unpack_dual(out).tangent is not None
     assert kernels.calls == 0
+
+
+def _as_torch_clips(grads, max_norm=1.0):
+    """(norm, gradients) of torch's clip on copies of the same layout"""
+    params = _with_grads(*[torch.empty_strided(g.shape, g.stride(), dtype=g.dtype).copy_(g) for g in grads])
+    return torch.nn.utils.clip_grad_norm_(params, max_norm), [p.grad for p in params]
+
+
+@pytest.mark.parametrize("what", ["float64", "float64 among others", "sparse"])
+@pytest.mark.parametrize("error_if_nonfinite", [False, True])
+def test_what_the_kernels_do_not_take_is_clipped_by_torch(kernels, what, error_if_nonfinite):
+    grads = {"float64": [torch.randn(5).double(), torch.randn(2, 3).double()],
+             "float64 among others": [torch.randn(6), torch.randn(5).double(), torch.randn(4, 6)[:, :3]],
+             "sparse": [torch.eye(4).to_sparse().coalesce()]}[what]
+    if what == "sparse":
+        params = _with_grads(grads[0].clone())
+        try:
+            want = torch.nn.utils.clip_grad_norm_(_with_grads(grads[0].clone()), 1.0)
+        except Exception as refused:             # as torch has it
+            with pytest.raises(type(refused)):
+                optim.clip_grad_norm_(params, 1.0, error_if_nonfinite=error_if_nonfinite)
+        else:
+            assert float(optim.clip_grad_norm_(params, 1.0, error_if_nonfinite=error_if_nonfinite)) == float(want)
+    else:
+        want, clipped = _as_torch_clips(grads)
+        params = _with_grads(*grads)
+        norm = optim.clip_grad_norm_(params, 1.0, error_if_nonfinite=error_if_nonfinite)
+        assert torch.equal(norm, want) and all(torch.equal(p.grad, c) for p, c in zip(params, clipped))
+    assert kernels.calls == 0
+
+
+def test_a_distributed_gradient_is_clipped_by_torch(kernels):
+    """A tensor of several processes has no address of its own."""
+    import torch.distributed as dist
+    from nextou_amd import ddp
+    from torch.distributed.tensor import Shard, distribute_tensor, init_device_mesh
+    ddp.init_single_process_group("gloo")
+    try:
+        g = torch.randn(6, 4)
+        d = distribute_tensor(g, init_device_mesh("cpu", (1,)), [Shard(0)])
+        p = torch.nn.Parameter(torch.zeros_like(d))
+        p.grad = d.clone()
+        optim.clip_grad_norm_([p], 1.0)
+        assert torch.allclose(p.grad.full_tensor(), g / g.norm(), atol=1e-6)
+        with pytest.raises(TypeError):
+            optim.grad_norm([d])
+    finally:
+        dist.destroy_process_group()
+    assert kernels.calls == 0
+
+
+def test_train_step_clips_float64_parameters_with_another_optimizer(kernels):
+    """The trainer's step of an optimizer without a clip of its own, as it ran on torch's clip"""
+    from nextou_amd import harness
+    net = torch.nn.Linear(4, 3).double()
+    trainer = object.__new__(harness.StandaloneTrainerBase)
+    trainer.network, trainer.optimizer = net, torch.optim.SGD(net.parameters(), 0.5)
+    trainer.loss = lambda out, target: ((out - target) ** 2).sum() * 1e3
+    x, t = torch.randn(6, 4).double(), torch.randn(6, 3).double()
+    before = [p.detach().clone() for p in net.parameters()]
+    trainer.train_step(x, t)
+    moved = torch.cat([((a - b) / 0.5).flatten() for a, b in zip(before, [p.detach() for p in net.parameters()])])
+    assert abs(float(moved.norm()) - 12.0) < 1e-4
