@@ -27,6 +27,7 @@ import operator
 import os
 from typing import Iterable, List, Optional, Union
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -140,12 +141,51 @@ def _norm_rows(tensors: List[torch.Tensor], in_place: bool):
         if not _flat_run(t):
             if in_place and any(a < b for a, b in _strides_and_reach(t)):
                 raise ValueError("gradient norm: a gradient of shape %s and strides %s overlaps itself" % (tuple(t.shape), t.stride()))
-            if in_place and any(t.data_ptr() == c.data_ptr() for c, _ in copies):
-                raise RuntimeError("gradient norm: two of the gradients share memory (the same one listed twice?)")
             copies.append((t, t.contiguous()))
-            t = copies[-1][1]
-        vals.extend((t.data_ptr(), n, code))
+            vals.extend((copies[-1][1].data_ptr(), n, code))
+        else:
+            vals.extend((t.data_ptr(), n, code))
+    if in_place and copies:                   # (the library compares the dense ones)
+        _check_strided_apart(tensors, copies)
     return vals, copies
+
+
+def _check_strided_apart(tensors: List[torch.Tensor], copies) -> None:
+    """RuntimeError where an element of a strided gradient is another gradient's as well."""
+    strided = {id(t) for t, _ in copies}
+    spans = sorted(((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum(s * (n - 1) for s, n in zip(t.stride(), t.shape))), i, t)
+                    for i, t in enumerate(tensors) if t.numel()), key=operator.itemgetter(0, 1, 2))
+    open_spans = []
+    for lo, hi, _, t in spans:
+        open_spans = [(h, o) for h, o in open_spans if h > lo]
+        for _, o in open_spans:
+            if (id(t) in strided or id(o) in strided) and _share_memory(t, o):
+                raise RuntimeError("gradient norm: two of the gradients share memory (the same one listed twice?)")
+        open_spans.append((hi, t))
+
+
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors whose spans meet have a byte in common.  Column blocks of one wide tensor are told apart by their addresses modulo
+    the row's length; anything else element by element."""
+    row = max([s * t.element_size() for t in (a, b) for s, n in zip(t.stride(), t.shape) if n > 1], default=1)
+    blocks = []
+    for t in (a, b):
+        size = t.element_size()
+        lo = t.data_ptr() % row
+        blocks.append((lo, lo + size + sum(s * size * (n - 1) for s, n in zip(t.stride(), t.shape) if s * size % row)))
+    (lo_a, hi_a), (lo_b, hi_b) = blocks
+    if max(hi_a, hi_b) <= row and (hi_a <= lo_b or hi_b <= lo_a):
+        return False
+    return bool(np.intersect1d(_addresses(a), _addresses(b)).size)
+
+
+def _addresses(t: torch.Tensor) -> np.ndarray:
+    """Of every pair of bytes of a float32, bfloat16 or float16 tensor"""
+    size = t.element_size()
+    at = np.arange(t.data_ptr(), t.data_ptr() + size, 2, dtype=np.int64)
+    for s, n in zip(t.stride(), t.shape):
+        at = (at[:, None] + np.arange(n, dtype=np.int64) * (s * size)).reshape(-1)
+    return at
 
 
 def _strides_and_reach(t: torch.Tensor):

@@ -163,3 +163,29 @@ def test_train_step_clips_float64_parameters_with_another_optimizer(kernels):
     trainer.train_step(x, t)
     moved = torch.cat([((a - b) / 0.5).flatten() for a, b in zip(before, [p.detach() for p in net.parameters()])])
     assert abs(float(moved.norm()) - 12.0) < 1e-4
+
+
+def test_strided_gradients_that_share_an_element_are_refused(kernels):
+    base = torch.randn(12, 16)
+    apart = [
+        [base[:, :4], base[:, 4:8], base[:, 8:]], [base[::2, :4], base[1::2, :4]], [base[:6, ::2], base[:6, 1::2]], [base[2:5, 3:6], base[5:9, 3:6]],
+        [base[:, :4], base[3, 4:16]], [base[:, 1], base[:, 2]], [base.t()[:4], base[:, 4:]], [base[:, :4], base[:, 5:6], torch.randn(3)],
+        [base[:, 14:], base.view(-1)[16:30]], [base.view(-1)[0:64:4], base.view(-1)[1:64:4]],
+    ]
+    share = [
+        [base[:, :4], base[:, 2:6]], [base[:, :4], base[::3, 3:5]], [base[:, :4], base], [base[:, 4:8], base.view(-1)[7:9]], [base[1:, :4], base[:-1, :4]],
+        [base[:, :4].t(), base[:, 3]], [base.view(-1)[0:64:4], base.view(-1)[2:64:6]], [base[:, :4], torch.randn(3), base[:, :4]],
+        [base[:, :4], base[0, 0]], [base.view(torch.bfloat16)[:, 1:4], base[:, 1:3]],
+    ]
+    for views in apart:
+        grads = [v.clone() for v in views]
+        want = math.sqrt(sum(float((v.double() ** 2).sum()) for v in grads))
+        optim.clip_grad_norm_(_with_grads(*views), want / 2)
+        assert all(torch.allclose(v, g / 2, rtol=1e-5) for v, g in zip(views, grads))
+    before = base.clone()
+    for views in share:
+        for order in (views, views[::-1]):
+            with pytest.raises(RuntimeError, match="share memory"):
+                optim.clip_grad_norm_(_with_grads(*order), 1e-3)
+    assert torch.equal(base, before)
+    assert float(optim.grad_norm([base[:, :4], base[:, 2:6]])) > 0          # a norm only reads
