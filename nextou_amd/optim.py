@@ -139,7 +139,7 @@ def _norm_rows(tensors: List[torch.Tensor], in_place: bool):
         if not t.data_ptr():
             raise _OtherTypes("gradient norm: a %s without memory of its own" % type(t).__name__)
         if not _flat_run(t):
-            if in_place and any(a < b for a, b in _strides_and_reach(t)):
+            if in_place and any(a < b for a, b in _strides_and_reach(t)) and _overlaps_itself(t):
                 raise ValueError("gradient norm: a gradient of shape %s and strides %s overlaps itself" % (tuple(t.shape), t.stride()))
             copies.append((t, t.contiguous()))
             vals.extend((copies[-1][1].data_ptr(), n, code))
@@ -188,8 +188,12 @@ def _addresses(t: torch.Tensor) -> np.ndarray:
     return at
 
 
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    return any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)) or np.unique(_addresses(t)).size * 2 != t.numel() * t.element_size()
+
+
 def _strides_and_reach(t: torch.Tensor):
-    """Per dimension longer than one, by ascending stride: (stride, elements that the smaller dimensions span); a stride below the span overlaps."""
+    """Per dimension longer than one, by ascending stride: (stride, elements that the smaller dimensions span); a stride below the span may overlap."""
     reach = 1
     for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         yield stride, reach

@@ -189,3 +189,13 @@ def test_strided_gradients_that_share_an_element_are_refused(kernels):
                 optim.clip_grad_norm_(_with_grads(*order), 1e-3)
     assert torch.equal(base, before)
     assert float(optim.grad_norm([base[:, :4], base[:, 2:6]])) > 0          # a norm only reads
+
+
+def test_interleaved_dimensions_without_a_common_element_are_taken(kernels):
+    base = torch.randn(12)
+    view = base.as_strided((2, 3), (3, 2))                     # elements 0, 2, 4, 3, 5, 7
+    want, around = view.clone(), base[[1, 6, 8, 9, 10, 11]].clone()
+    optim.clip_grad_norm_(_with_grads(view), float(want.norm()) / 2)
+    assert torch.allclose(view, want / 2, rtol=1e-5) and torch.equal(base[[1, 6, 8, 9, 10, 11]], around)
+    with pytest.raises(ValueError, match="overlaps itself"):
+        optim.clip_grad_norm_(_with_grads(base.as_strided((2, 3), (4, 2))), 1.0)
