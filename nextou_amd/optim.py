@@ -225,6 +225,7 @@ def _multi_norm(tensors: List[torch.Tensor], code: int, max_norm: float, scale: 
         if scale:
             for t, dense in copies:
                 t.copy_(dense)
+            torch.autograd.graph.increment_version(tensors)      # written by address: a graph that saved one of them has to notice
     return out
 
 
@@ -445,6 +446,8 @@ class ClipSGD(torch.optim.SGD):
                                                     0.0 if lr_dev else float(lr), lr_dev, float(group["momentum"]),
                                                     float(group["weight_decay"]), int(bool(group["nesterov"])), stream),
                            "clip_sgd_update")
+        written = [p for gi, _ in live for p in self.param_groups[gi]["params"] if p.grad is not None]
+        torch.autograd.graph.increment_version(written + [p.grad for p in written])      # written by address: graphs that saved them notice
         return norm
 
     def step(self, closure=None):

@@ -199,3 +199,34 @@ def test_interleaved_dimensions_without_a_common_element_are_taken(kernels):
     assert torch.allclose(view, want / 2, rtol=1e-5) and torch.equal(base[[1, 6, 8, 9, 10, 11]], around)
     with pytest.raises(ValueError, match="overlaps itself"):
         optim.clip_grad_norm_(_with_grads(base.as_strided((2, 3), (4, 2))), 1.0)
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_a_graph_that_saved_a_gradient_notices_the_clip(kernels, strided):
+    x = torch.randn(6, 4, requires_grad=True)
+    (g,) = torch.autograd.grad((x ** 3).sum(), (x,), create_graph=True)
+    if strided:
+        g = torch.cat([g, g], 1)[:, 1:5]
+    penalty = (g ** 2).sum()                                   # saves g
+    params = _with_grads(g.detach())
+    optim.grad_norm([p.grad for p in params])                  # only reads
+    penalty.backward(retain_graph=True)
+    optim.clip_grad_norm_(params, 1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        penalty.backward()
+
+
+def test_a_graph_that_saved_a_parameter_notices_the_step(monkeypatch):
+    """ClipSGD's own kernels, over two parameter groups"""
+    from test_linear_act_host import _StandInLib as StepLib
+    fake = StepLib()
+    monkeypatch.setattr(_lib, "lib", lambda: fake)
+    a, b = torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(4))
+    opt = optim.ClipSGD([{"params": [a], "lr": 0.5}, {"params": [b], "lr": 0.25}], 0.1)
+    opt._device_type = "cpu"
+    loss = (a * b).sum()
+    loss.backward(retain_graph=True)
+    opt.clip_and_step(1.0)
+    assert opt.last_path == "own"
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
