@@ -62,7 +62,7 @@ __device__ __forceinline__ void activate(float (&f)[E], int act, float slope) {
         }
     } else if (act == kActHardswish) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) f[i] = f[i] * fminf(fmaxf(f[i] + 3.f, 0.f), 6.f) * (1.f / 6.f);
+        for (int i = 0; i < E; ++i) f[i] *= fminf(fmaxf(f[i] + 3.f, 0.f), 6.f) * (1.f / 6.f);      // (6 times a large z would leave the range)
     }
 }
 
