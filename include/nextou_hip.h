@@ -598,8 +598,9 @@ int nextou_stem_bwd(const float* x, const float* gy, const uint32_t* act_mask, c
  *   z[p, g*N + n] = sum_k x[p, g*K + k] * w[g*N + n, k] + bias[g*N + n]        y = act(z) + residual
  *   act: 0 none, 1 relu, 2 leaky relu (slope), 3 gelu (z Phi(z)), 4 hardswish.  Any P, N, K >= 1, any element-aligned pointers and row
  *   strides (ldx and ldr may be 0: one row for all; ldy >= groups * N); P <= 2^36, and where a row of N or K is shorter
- *   than 16 bytes P * max(N, K, 64) < 2^36; columns are dense, w is dense (groups * N, K).  bias and residual may be NULL; bias
- *   is float32 when bias_f32, else of the rows' type.  Sums in float32, each output rounded once.
+ *   than 16 bytes P * max(N, K, 64) < 2^36; rows that no launch holds are refused (P * ceil(N / 64) < 2^30 always fits); columns are
+ *   dense, w is dense (groups * N, K).  bias and residual may be NULL; bias is float32 when bias_f32, else of the rows' type.  Sums in
+ *   float32, each output rounded once.
  *   pre (may be NULL): z for the backward, dense (P, groups * N) — float32 for float32 rows, float16 for both 16-bit types, clamped to
  *   its range, a positive z never rounded to zero.
  * nextou_linear_act_bwd   dz = gy * act'(z) (rounded to the rows' type for the products, unrounded in gb), gx = dz w, gw = dz^T x,

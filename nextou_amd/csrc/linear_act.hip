@@ -523,16 +523,19 @@ __global__ __launch_bounds__(64 * WR * WC, (BM / WR) * (BN / WC) > 128 * 64 ? 1 
 }
 
 template <typename T, int BM, int BN, int WR, int WC, int DMA>
-void launch_rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
-                      hipStream_t s) {
+int launch_rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
+                     hipStream_t s) {
     const int mt = (int)cdiv64(M, BM), nt = cdiv(N, BN);
     const size_t lds = (size_t)(BM + BN) * CH * 16 * NBUF;
     auto* kernel = &rows_gemm_kernel<T, BM, BN, WR, WC, DMA>;
     if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    const int64_t items = (int64_t)mt * nt;
-    const dim3 grid((unsigned)(cdiv64(items, kXcds) * kXcds), (unsigned)groups);
+    const int64_t blocks = cdiv64((int64_t)mt * nt, kXcds) * kXcds;
+    // (rows of a stride of 0 make such calls possible: their number is not bound by the memory that x takes)
+    NEXTOU_REQUIRE(blocks * 64 * WR * WC < (1ll << 32), "linear_act: %ld rows of %d columns are more than one launch takes", M, N);
+    const dim3 grid((unsigned)blocks, (unsigned)groups);
     hipLaunchKernelGGL((rows_gemm_kernel<T, BM, BN, WR, WC, DMA>), grid, dim3(64 * WR * WC), lds, s, A, B, out, M, N, K, lda, ldb, ldo, bg,
                        mt, nt, e);
+    return 0;
 }
 
 bool on16(const void* p, long ld, size_t size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (long)size % 16 == 0; }
@@ -1248,25 +1251,25 @@ int tile_size(long M, int N, int K, int groups, bool dma, size_t S) {
 }
 
 template <typename T>
-void rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
+int rows_gemm(const T* A, const T* B, T* out, long M, int N, int K, int groups, long lda, long ldb, long ldo, long bg, const Epilogue& e,
                hipStream_t s) {
     constexpr size_t S = sizeof(T);
     const bool dma = on16(A, lda, S) && on16(B, ldb, S) && (long)K * S % 16 == 0 && bg * (long)S % 16 == 0;
     const PanelPlan p = plan_panel(N, K, groups, S);
     if (p.ks && M >= kPanelRows) {
         panel_gemm<T>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, p, s);
-        return;
+        return 0;
     }
     if (few_rows(M, N, K, groups, S)) {
         launch_few_rows<T>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-        return;
+        return 0;
     }
     const int tile = tile_size(M, N, K, groups, dma, S);
-    if (tile == 256) launch_rows_gemm<T, 256, 256, 2, 4, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else if (dma && tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else if (dma) launch_rows_gemm<T, 64, 64, 2, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else if (tile == 128) launch_rows_gemm<T, 128, 128, 2, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
-    else launch_rows_gemm<T, 64, 64, 2, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    if (tile == 256) return launch_rows_gemm<T, 256, 256, 2, 4, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    if (dma && tile == 128) return launch_rows_gemm<T, 128, 128, 2, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    if (dma) return launch_rows_gemm<T, 64, 64, 2, 2, 1>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    if (tile == 128) return launch_rows_gemm<T, 128, 128, 2, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
+    return launch_rows_gemm<T, 64, 64, 2, 2, 0>(A, B, out, M, N, K, groups, lda, ldb, ldo, bg, e, s);
 }
 
 // The weight gradient's tiles and split: 128-column tiles, 64 where a side is that small, 256 (16 bits, aligned rows) where those alone give
@@ -1366,7 +1369,7 @@ BwdPlan plan_bwd(int64_t P, int N, int K, int groups, int dtype, int act, bool w
 
 template <typename T>
 int launch_fwd(const T* x, const T* w, T* y, int64_t P, int N, int K, int groups, int64_t ldx, int64_t ldy, const Epilogue& e, hipStream_t s) {
-    rows_gemm<T>(x, w, y, P, N, K, groups, ldx, K, ldy, (long)N * K, e, s);
+    if (int r = rows_gemm<T>(x, w, y, P, N, K, groups, ldx, K, ldy, (long)N * K, e, s)) return r;
     return check_launch("linear_act_fwd");
 }
 
@@ -1394,7 +1397,8 @@ int launch_bwd(const T* gy, const T* x, const T* w, const void* saved, int kind,
     if (gx) {
         const Epilogue none{};
         // the zeros behind N in dz and in wt's rows are multiplied along: whole pieces
-        rows_gemm<T>(gy, wt, gx, P, K, padded && groups == 1 ? b.ldt : N, groups, ldg, b.ldt, (long)groups * K, (long)K * b.ldt, none, s);
+        if (int r = rows_gemm<T>(gy, wt, gx, P, K, padded && groups == 1 ? b.ldt : N, groups, ldg, b.ldt, (long)groups * K, (long)K * b.ldt, none, s))
+            return r;
     }
     const int splits = gw ? cols_gemm<T>(gy, x, gw, split, P, N, K, groups, ldg, ldx, padded, dtype, s) : 1;
     SplitSum first{}, second{};
