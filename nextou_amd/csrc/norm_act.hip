@@ -1350,6 +1350,7 @@ __global__ __launch_bounds__(kThreads) void bn_clw_bwd_reduce_kernel(const T* __
                 p[u].load(x + (r + (long long)u * t.nry) * C + t.ch0);
                 g[u].load(gy + (r + (long long)u * t.nry) * C + t.ch0);
             }
+            __builtin_amdgcn_sched_barrier(0);      // all four loads in flight: left alone the second row's wait for the first's (132 channels, 172032 rows: 49 us against 35)
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
