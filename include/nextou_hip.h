@@ -592,9 +592,10 @@ int nextou_stem_bwd(const float* x, const float* gy, const uint32_t* act_mask, c
 
 /* ------------------------------------------------------------------------------------------
  * K10  point-wise products with their epilogue (ABI v15): the 1x1 convolution / linear layer of a block with its bias, its activation
- * and its shortcut in one launch, and the gradients, in float32 (dtype 0), bfloat16 (1) and float16 (2).  Replaces conv -> act (-> add)
+ * and its shortcut in one launch, and the gradients, in float32 (dtype 0), bfloat16 (1) and float16 (2).  What it computes is conv -> act (-> add)
  * of the reference's BasicConv without a norm (torch_nn.py:66-92) and, with the norm's running statistics folded into w and bias,
- * conv -> norm -> act (-> add) of FFN / fc1 / fc2 in evaluation (NexToU_Encoder_Decoder.py:368-390, :710-720, :833-842).
+ * conv -> norm -> act (-> add) of FFN / fc1 / fc2 in evaluation (NexToU_Encoder_Decoder.py:368-390, :710-720, :833-842); the modules of this
+ * package stay on K7 and the library there, a caller takes K10 through graph_ops.linear_act / pointwise_act.
  *   z[p, g*N + n] = sum_k x[p, g*K + k] * w[g*N + n, k] + bias[g*N + n]        y = act(z) + residual
  *   act: 0 none, 1 relu, 2 leaky relu (slope), 3 gelu (z Phi(z)), 4 hardswish.  Any P, N, K >= 1, any element-aligned pointers and row
  *   strides (ldx and ldr may be 0: one row for all; ldy >= groups * N); P <= 2^36, and where a row of N or K is shorter
@@ -603,9 +604,10 @@ int nextou_stem_bwd(const float* x, const float* gy, const uint32_t* act_mask, c
  *   float32, each output rounded once.
  *   pre (may be NULL): z for the backward, dense (P, groups * N) — float32 for float32 rows, float16 for both 16-bit types, clamped to
  *   its range, a positive z never rounded to zero.
- * nextou_linear_act_bwd   dz = gy * act'(z) (rounded to the rows' type for the products, unrounded in gb), gx = dz w, gw = dz^T x,
+ * nextou_linear_act_bwd   dz = gy * act'(z) (rounded to the rows' type for the products — in float16 a slope above 1 can take it past 65504, to
+ *   infinity, and a small one into the subnormals — unrounded in gb), gx = dz w, gw = dz^T x,
  *   gb = sum_p dz; any of gx (dense), gw (dense, like w), gb (float32 when gb_f32, else the rows' type) may be NULL.  saved_kind: 0 none
- *   (act 0), 1 `saved` is the forward's pre, 2 `saved` is the forward's y, dense (relu, leaky relu with slope >= 0 and no residual: its sign is z's).
+ *   (act 0), 1 `saved` is the forward's pre, 2 `saved` is the forward's y, dense (relu, leaky relu with slope >= 0 and no residual: its sign is z's; a bfloat16 y of a positive z below 2^-134 is 0 and counts as such).
  *   Sums over points in a fixed order: bit-reproducible.
  * workspace (backward): nextou_linear_act_bwd_workspace's bytes, contents irrelevant; one per call in flight.
  * ---------------------------------------------------------------------------------------- */

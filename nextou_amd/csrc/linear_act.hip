@@ -189,8 +189,8 @@ template <typename T>
 __device__ __forceinline__ u32x4 load_tail(const T* row, long c, long C) {
     return load16(row + min(c, C - Num<T>::E));
 }
-// (In 32-bit steps: with 64-bit shifts by a register the compiler put the shift count into the last register of the kernel's allocation,
-// and the results were wrong now and then — garbage in about one of thirty runs of the float32 few_rows_kernel, gone with these.)
+// (In 32-bit steps.  A form with 64-bit shifts by a register stood in a build whose float32 few_rows_kernel gave wrong results in about one of thirty
+// runs; this form and another LDS layout came in one step, and the results have been right since.  Which of the two it was is not known.)
 template <typename T>
 __device__ __forceinline__ u32x4 tail_fixed(u32x4 v, long c, long C) {
     constexpr int E = Num<T>::E;
@@ -224,7 +224,8 @@ __device__ __forceinline__ u32x4 tail_fixed(u32x4 v, long c, long C) {
 // Epilogue: the sums go through LDS (the wave's own part of it, 32 rows at a time) so that a lane then holds E consecutive columns of a
 // row: bias, activation, residual and the stores are 16-byte accesses of whole lines.
 //
-// Bound by the LDS reads beside the matrix unit, and by the clock, which falls to 1.7-1.8 GHz in long products.  Measured: 8192^3 bfloat16 971 us =
+// In long products the matrix unit is busy 55 % of the cycles, at a clock that falls to 1.6-1.8 GHz; the waves wait a third of their cycles, 2 % of
+// them for LDS, the rest at the stage barriers for loads (8192 x 4096 -> 4096 fetches its operands four times).  Measured: 8192^3 bfloat16 971 us =
 // 1130 TFLOP/s, 16384 x 2048 -> 8192 with gelu and z written 642 us, 8192 x 4096 -> 4096 float16 with hardswish 266 us = 1030 TFLOP/s; a library
 // product alone of these sizes takes 790, 464 and 191 us.  256 x 128 tiles, four waves of 128 x 128, and four shorter stages in LDS were slower.
 __device__ u32x4 g_zero_piece;      // stays zero
@@ -548,7 +549,8 @@ bool on16(const void* p, long ld, size_t size) { return reinterpret_cast<uintptr
 // k is put in the tile's rows, so a lane ends up with consecutive k and the epilogue above stores whole lines of the weight's layout.
 // p is split over blockIdx.z when there are few tiles: float32 partial blocks, added in a fixed order by split_sum_kernel.
 // Measured: 16384 rows, 8192 x 2048 bfloat16 612 us = 900 TFLOP/s (256 tiles; 776 us with 128); 21504 rows, 1056 x 264 67 us = 179 TFLOP/s, where
-// 3 x 9 tiles of 128 hold 264 x 1056 columns to 69 % and 486 workgroups read x nine times and dz three times.
+// 3 x 9 tiles of 128 hold 264 x 1056 columns to 69 % and 486 workgroups read x nine times and dz three times: 192 MB come from memory for 57, the
+// waves wait half of their cycles.
 template <typename T, int BC>
 __device__ __forceinline__ int col_swizzle(int row, int piece) {
     if constexpr (sizeof(T) == 4) return piece;
@@ -823,7 +825,9 @@ __device__ __forceinline__ void transpose_weight(T (&tile)[64][66], const T* __r
 // dz = gy act'(saved) as dense rows of ld_dz columns (a multiple of 16 bytes, so that both products fetch it without registers; the columns
 // behind C are zeros), and per-workgroup column sums of the unrounded dz.  A workgroup holds `lanes` 16-byte pieces of a row and 256 / lanes
 // rows at a time; the pieces walk fastest over the workgroups.  Reads gy and the saved tensor, writes dz: HBM-bound
-// (21504 x 1056 bfloat16 with gelu: 136 MB in 40 us, 3.4 TB/s).  The weight is transposed by the workgroups behind `act_blocks`, in the same
+// (21504 x 1056 bfloat16 with gelu: 136 MB in 40 us, 3.4 TB/s).  The rounding of dz to 16 bits is the matrix units': the gradients of a bfloat16
+// layer are 0.0023 off the 64-bit ones in norm, where the rounding of the outputs alone gives 0.0017; a second 16-bit part would double both
+// products.  The weight is transposed by the workgroups behind `act_blocks`, in the same
 // launch (5 us less than in one of its own).
 // KIND 0: no activation (only the sums), 1: saved is z, 2: saved is y and only its sign matters
 template <typename T, int KIND>
@@ -899,8 +903,9 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const T* __restrict__ gy,
 // Panel rows lie an odd number of pieces apart, so that eight consecutive rows fall on all banks.
 // Results stay in registers: the lane halves of a 32 x 32 tile hold alternate groups of four columns; in 16 bits an exchange between the
 // halves makes that eight consecutive columns, so residual, z and output move as 16-byte pieces.
-// Bound by memory, mostly by the stores (output lines are completed by two waves' worth of 16-byte pieces): 172032 rows 132 -> 528 bfloat16 86 us =
-// 2.65 TB/s, 6 groups of 44 -> 44 float32 120 us = 3.0 TB/s; a copy reaches 4.9.  1024 threads, two tiles at a time, output lines gathered in LDS,
+// 172032 rows 132 -> 528 bfloat16 87 us = 2.6 TB/s, 6 groups of 44 -> 44 float32 120 us = 3.0 TB/s; a copy reaches 4.9.  No unit is full (bfloat16: VALU
+// 37 % of the cycles, matrix unit 15, waves waiting 26; float32 24, 38, 20), and 10-14 % more is written than the output (lines that two 16-byte
+// pieces of different waves complete).  1024 threads, two tiles at a time, output lines gathered in LDS,
 // and stores past the caches (215 us) were no faster.
 // KS: k steps (two pieces each), zeros behind K; LOW: the steps that are whole in every K of this size.
 template <int E, int N>

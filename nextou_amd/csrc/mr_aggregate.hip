@@ -96,9 +96,9 @@ __global__ __launch_bounds__(512) void mr_fwd_lds_kernel(
 //     64-byte stores); with stores, bank conflicts, arg tracking and staging all switched off it still needed 43 us.
 // Here: no cross-lane step at all; the ids of a query are loaded once (dwordx4) and kept as LDS byte addresses (id << shift, the
 // workgroup's QUADS = 1, 2 or 4 quads of a point are adjacent: tile4[m * QUADS + q], so the quad is an immediate of the ds_read);
-// two v_pk_add_f32 form the four differences of a gather; the (max, arg) update is one 12-instruction block (mr_update4);
-// every global access is a 256-byte row segment (64 consecutive queries of one channel).  1.03e7 VALU wave-instructions, 36 us
-// = 0.30 of 8 TB/s at that shape; what remains is 17 us of VALU issue and 18 us of LDS time (74 % bank-conflict cycles: 16 lanes
+// four v_sub_f32 form the four differences of a gather; the (max, arg) update is one 12-instruction block (mr_update4);
+// every global access is a 256-byte row segment (64 consecutive queries of one channel).  1.18e7 VALU wave-instructions, 36 us
+// = 0.30 of 8 TB/s at that shape; what remains is 19 us of VALU issue and 18 us of LDS time (74 % bank-conflict cycles: 16 lanes
 // of a ds_read_b128 pick among 16 bank groups at random) that overlap only partly.
 // grid = (n_tiles, quad blocks, B); LDS = QUADS * M float4; K <= KB * NB.
 // ---------------------------------------------------------------------------------------------

@@ -1860,11 +1860,11 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
     x (..., groups * K); weight (groups * N, K); bias (groups * N,) or None; residual (..., groups * N) or None -> (..., groups * N).
     ``groups`` > 1: channel group g of the output sees channel group g of the input, as in a grouped 1x1 convolution.  ``act``: "none",
-    "relu", "leakyrelu" (``negative_slope``), "gelu" (the exact one) or "hswish".
+    "relu", "leakyrelu" (``negative_slope``), "gelu" (the exact one) or "hswish" (also "hardswish").
 
     float32, bfloat16 or float16; all tensors of one type, except that the bias may be float32 beside 16-bit rows.  Sums are held in
     float32 and every output and gradient is rounded once (with an activation in 16 bits, so is d loss / d z on its way into the two
-    gradient products).  Under autocast the tensors are cast to the autocast type first.  Any sizes and any strides: columns that are not
+    gradient products: the matrix units read 16 bits; in float16 a slope above 1 can take it past 65504, to infinity).  Under autocast the tensors are cast to the autocast type first.  Any sizes and any strides: columns that are not
     dense are copied, an expanded row is read as it is.  Gradients are bit-reproducible; there is no double backward and no forward-mode
     derivative (NotImplementedError for a tensor with a tangent).
     ValueError / TypeError for shapes, types or devices that do not fit."""

@@ -15,7 +15,7 @@ torch's implementation, unchanged — ``last_path`` / ``last_reason`` say which 
 than its parameter is copied into the parameter's order first.
 
 ``clip_grad_norm_`` and ``grad_norm`` are the clip alone, for any optimizer: gradients of float32, bfloat16 and float16 in one list, the 2-, 1-
-or maximum norm, two launches whatever the tensor count (csrc/grad_norm.hip, ABI v15).
+or maximum norm, two launches and one more for every 224 tensors of a list longer than that (csrc/grad_norm.hip, ABI v15).
 """
 from __future__ import annotations
 
@@ -247,7 +247,7 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: f
 @torch.no_grad()
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False, foreach: Optional[bool] = None) -> torch.Tensor:
-    """``torch.nn.utils.clip_grad_norm_`` for gradients on the GPU in two launches: every gradient times ``min(1, max_norm / (norm + 1e-6))``, in place,
+    """``torch.nn.utils.clip_grad_norm_`` for gradients on the GPU in two launches (and one for every 224 of more than 224 tensors): every gradient times ``min(1, max_norm / (norm + 1e-6))``, in place,
     rounded once; returns the norm before the clip (0-dim float32, no host synchronisation unless ``error_if_nonfinite``).
 
     Gradients may be float32, bfloat16 and float16 in one list, of any dense layout (others are copied and written back).  A norm that is
