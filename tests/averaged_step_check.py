@@ -76,9 +76,8 @@ def main():
     ap.add_argument("--workload", default="tiny")
     ap.add_argument("--steps", type=int, default=3)
     ap.add_argument("--captured-collectives", action="store_true",
-                    help="also run the averaged step CAPTURED into a hipGraph (RCCL collectives inside the capture): the explicit opt-in of "
-                         "bench.py --graph on, where PyTorch's RCCL watchdog thread can abort the process (DESIGN.md 6); without the flag the "
-                         "modes are the defaults of every N (eager averaged step, captured plain step)")
+                    help="also run the averaged step CAPTURED into a hipGraph (RCCL collectives inside the capture), where PyTorch's RCCL watchdog "
+                         "thread can abort the process: the averager refuses it; without the flag the modes are the defaults of every N (eager averaged step, captured plain step)")
     args = ap.parse_args()
     _lib.lib()
     torch.cuda.set_device(DEV)

@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 def _xfail_on_watchdog_capture_error(proc):
     """The one failure of these runs that is neither this repository's nor deterministic: PyTorch's RCCL watchdog THREAD terminating the process
     with hipErrorCapturedEvent while a step with collectives is being captured (about once in 25 runs of the tiny workload,
-    two precautions in place, mechanism not established — tools/rccl_capture_watchdog_repro.py stayed clean).  Reported as XFAIL with this
+    two precautions in place, mechanism not established — a stand-alone attempt stayed clean).  Reported as XFAIL with this
     reason (no retry, no skip; the outcome stays visible in the report) — every other failure fails the test."""
     err = proc.stderr or ""
     if proc.returncode != 0 and "hipErrorCapturedEvent" in err and "watchdog thread terminated" in err:
