@@ -1232,7 +1232,8 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // The panel kernel from 65536 rows on: then each of its 2048 waves has 32 rows.  Panel against tiles, us: 65536 rows bfloat16 132 -> 132 15.5 / 27.8,
 // 264 -> 528 48 / 69; 172032 rows 132 -> 528 91 / 164, float32 249 / 330; fewer rows leave waves idle, 21504 rows 132 -> 264 17.4 / 16.0, float32
-// 132 -> 132 34 / 20.  Rows of more than 17 k steps leave no registers for the next rows: 172032 rows 384 -> 384 132 / 117, 400 -> 1600 593 / 484.
+// 132 -> 132 34 / 20.  Wide ones: 65536 rows 264 -> 2112 128 / 211, 132 -> 4096 169 / 380, float32 132 -> 4096 868 / 857; the panels of long rows are
+// narrow, each reads all of x again: 264 -> 4096 421 / 390, 172032 rows 1119 / 982 (not worth a rule of its own).  Rows of more than 17 k steps leave no registers for the next rows: 172032 rows 384 -> 384 132 / 117, 400 -> 1600 593 / 484.
 constexpr long kPanelRows = 65536;
 // k split over the waves where fewer than 64 tiles of 64 x 64 would be there, and up to 160 with rows of 4 KB and more.  Split against tiles, us:
 // bfloat16 336 rows 528 -> 528 5.9 / 7.0, 1000 rows 132 -> 132 5.0 / 6.2, 256 rows 2048 -> 2048 14.0 / 19.7; 700 rows 528 -> 528 10.9 / 7.3,
